@@ -431,6 +431,90 @@ int tc_adagrad(int dtype, size_t n, void *p, const void *g, void *total, double 
 int tc_rmsprop(int dtype, size_t n, void *p, const void *g, void *mean_square, double rate,
                double decay, double eps, void *stream);
 
+/* ---- training operators (no counterpart in the reference) ---------------- */
+/* What a training step over a vocabulary needs beside the products and the
+ * optimizers: layer norm, the log probabilities of its tokens, the clipping
+ * of its gradients.  Rows are `stride` elements apart (their elements side by
+ * side), with at least as many elements as the row has; sums and statistics
+ * are f32 (the norm's f64), each result is rounded once, to its type. */
+
+/* y = (x - mean) * rstd * weight + bias for each of `rows` rows of `cols`
+ * elements, rstd = 1/sqrt(mean((x - mean)^2) + eps).  weight and bias (each
+ * may be NULL: one, zero) hold `cols` values of `param_dtype`, which is
+ * `dtype` or TC_F32.  statistics (may be NULL) receives (mean, rstd) of each
+ * row, for the backward pass; it starts on an 8-byte boundary.  y may be x
+ * (with the same stride). */
+int tc_layer_norm(int dtype, int param_dtype, size_t rows, size_t cols, const void *x, size_t x_stride,
+                  const void *weight, const void *bias, double eps, void *y, size_t y_stride, float *statistics,
+                  void *stream);
+/* The gradients of tc_layer_norm from the gradient `grad` of y and the
+ * forward pass's x and statistics: grad_x (may be grad or x, with the same
+ * stride), and grad_weight and grad_bias of `param_dtype`, summed over the
+ * rows in an order that depends on the sizes alone.  Any of the three may be
+ * NULL: it is not computed.  The sums use the stream's scratch. */
+int tc_layer_norm_backward(int dtype, int param_dtype, size_t rows, size_t cols, const void *grad,
+                           size_t grad_stride, const void *x, size_t x_stride, const float *statistics,
+                           const void *weight, void *grad_x, size_t grad_x_stride, void *grad_weight,
+                           void *grad_bias, void *stream);
+
+/* A position that holds no token (padding, a prompt's part of a loss): its
+ * logprob is 0 and no gradient flows through it. */
+#define TC_NO_TOKEN 0xFFFFFFFFu
+/* The largest `top` of tc_token_logprobs. */
+#define TC_MAX_TOP 32
+/* For each of `rows` rows of `vocab` logits, all in f32, each output computed
+ * only where its pointer is not NULL:
+ *   logprobs    log(softmax(row)) at the row's token (a TC_NO_TOKEN gives 0,
+ *               any other index past the vocabulary NaN);
+ *   entropy     -sum(p log p);
+ *   statistics  (m, log sum exp(x - m)), m the largest logit: what the
+ *               backward pass needs, and together the row's log-sum-exp;
+ *   top_tokens, top_logprobs  the `top` likeliest tokens [rows x top] and
+ *               their log probabilities, the likeliest first, of equal ones
+ *               the lower index first; NaNs rank last.
+ * Logits of -inf have probability zero.  A row of nothing else has the
+ * statistics (-inf, 0), the logprob -inf and the entropy 0.  A NaN or +inf
+ * in a row makes its logprob and entropy NaN. */
+int tc_token_logprobs(int dtype, size_t rows, size_t vocab, const void *logits, size_t row_stride,
+                      const uint32_t *tokens, float *logprobs, float *entropy, float *statistics, uint32_t top,
+                      uint32_t *top_tokens, float *top_logprobs, void *stream);
+/* The logits' gradient from that of the logprobs and of the entropies (each
+ * may be NULL: zero):
+ *   grad_logprobs * ([j = token] - p_j) - grad_entropy * p_j * (log p_j + entropy)
+ * with the forward pass's statistics, and its entropy where grad_entropy is
+ * given.  A row whose two gradients are zero (or whose token is TC_NO_TOKEN
+ * or past the vocabulary, for the first) is written as zeros whatever its
+ * logits; so is a row of nothing but -inf.  grad_logits may be the logits
+ * (with the same stride). */
+int tc_token_logprobs_backward(int dtype, size_t rows, size_t vocab, const void *logits, size_t row_stride,
+                               const uint32_t *tokens, const float *statistics, const float *entropy,
+                               const float *grad_logprobs, const float *grad_entropy, void *grad_logits,
+                               size_t grad_stride, void *stream);
+/* Both at once, where the gradients are known before the logprobs are (a
+ * mean loss: -1/tokens each): the logits are read from memory once.
+ * logprobs, entropy and statistics may be NULL. */
+int tc_token_loss(int dtype, size_t rows, size_t vocab, const void *logits, size_t row_stride,
+                  const uint32_t *tokens, const float *grad_logprobs, const float *grad_entropy, float *logprobs,
+                  float *entropy, float *statistics, void *grad_logits, size_t grad_stride, void *stream);
+
+/* One gradient of a step: n elements of `dtype` side by side at g; clipped
+ * it goes to out (which may be g). */
+typedef struct tc_gradient {
+  const void *g;
+  void *out;
+  size_t n;
+  int dtype;
+} tc_gradient;
+/* norm[0] = the square root of the sum of every gradient's squares, in f64,
+ * added in an order that depends on the sizes alone, rounded once to f32.  `out` is not
+ * used.  Uses the stream's scratch. */
+int tc_grad_norm(const tc_gradient *grads, size_t count, float *norm, void *stream);
+/* out = g * min(1, limit / norm[0]), the factor in f32.  norm is read on the
+ * device, so a caller may first combine the norms of several ranks.  A norm
+ * of zero clips nothing, a NaN makes every gradient NaN.  Where the factor
+ * is one, gradients clipped in place are left alone. */
+int tc_clip_grads(const tc_gradient *grads, size_t count, const float *norm, double limit, void *stream);
+
 /* Status of bounded device-side waits since the library loaded: TC_ETIMEOUT
  * (and *fault = 1) if a tensor-core GEMM gave up waiting on its pipeline, or
  * a data-parallel step gave up waiting for another rank's flag, and

@@ -85,6 +85,16 @@ class AdamTensor(C.Structure):
     _fields_ = [("p", _p), ("g", _p), ("m", _p), ("v", _p), ("n", _sz)]
 
 
+class Gradient(C.Structure):
+    """tc_gradient: one tensor of a tc_grad_norm or tc_clip_grads call."""
+
+    _fields_ = [("g", _p), ("out", _p), ("n", _sz), ("dtype", C.c_int)]
+
+
+NO_TOKEN = 0xFFFFFFFF
+MAX_TOP = 32
+
+
 # name -> argtypes; every function returns int status.
 SIGNATURES = {
     "tc_last_error": [C.c_char_p, _sz],
@@ -152,6 +162,13 @@ SIGNATURES = {
     "tc_momentum": [_i, _sz, _p, _p, _p, _d, _d, _i, _p],
     "tc_adagrad": [_i, _sz, _p, _p, _p, _d, _d, _p],
     "tc_rmsprop": [_i, _sz, _p, _p, _p, _d, _d, _d, _p],
+    "tc_layer_norm": [_i, _i, _sz, _sz, _p, _sz, _p, _p, _d, _p, _sz, _p, _p],
+    "tc_layer_norm_backward": [_i, _i, _sz, _sz, _p, _sz, _p, _sz, _p, _p, _p, _sz, _p, _p, _p],
+    "tc_token_logprobs": [_i, _sz, _sz, _p, _sz, _p, _p, _p, _p, _u32, _p, _p, _p],
+    "tc_token_logprobs_backward": [_i, _sz, _sz, _p, _sz, _p, _p, _p, _p, _p, _p, _sz, _p],
+    "tc_token_loss": [_i, _sz, _sz, _p, _sz, _p, _p, _p, _p, _p, _p, _p, _sz, _p],
+    "tc_grad_norm": [_p, _sz, _p, _p],
+    "tc_clip_grads": [_p, _sz, _p, _d, _p],
     "tc_coalesce": [_u32, _szp, _u32, _szp, _u32p, _szp, _szp],
     "tc_device_status": [C.POINTER(_i)],
     "tc_device_status_reset": [],
