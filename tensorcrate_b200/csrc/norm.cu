@@ -113,79 +113,288 @@ __global__ void __launch_bounds__(1024) norm_rows_wide(const typename T::S *x, s
   }
 }
 
-// grad_x, and this block's share of grad_w and grad_b: a block walks its
-// rows and keeps the sums of the columns that its threads own in registers,
-// then writes them to its row of `partial` (w's sums, then b's).
-template <class T, class P, int E, int K>
-__global__ void __launch_bounds__(512) norm_grad_rows(const typename T::S *g, size_t g_stride,
-                                                      const typename T::S *x, size_t x_stride,
-                                                      const float2 *__restrict__ statistics,
-                                                      const typename P::S *__restrict__ w,
-                                                      typename T::S *dx, size_t dx_stride,
-                                                      float *__restrict__ partial, size_t rows, unsigned cols) {
-  using S = typename T::S;
-  __shared__ float room[2][2][32];
-  const unsigned t = threadIdx.x, threads = blockDim.x;
-  const float share = 1.0f / float(cols);
-  float sum_w[K * E], sum_b[K * E];
+// Copies 16 bytes from global to shared memory; a thread's copies complete in
+// the order of its commits.
+__device__ __forceinline__ void copy_async(uint32_t to, const void *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Until at most LEFT of this thread's last commits are under way.
+template <int LEFT> __device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// grad_x, and this block's share of grad_w and grad_b.  A block is `groups`
+// groups of `threads` threads; a group takes a turn of R neighbouring rows at
+// a time and its threads own the same columns of every row, so the columns'
+// sums stay in registers until the block adds its groups' and writes them to
+// its row of `partial` (w's sums, then b's).
+//
+// The rows come through a ring of DEPTH turns in shared memory, filled
+// asynchronously: HBM is not waited for once the ring runs, whatever few
+// threads the columns' sums leave room for.  A row is copied as the aligned
+// 16-byte granules that it touches (so rows that start anywhere are read at
+// full width; a granule that holds one valid byte can be read whole); E
+// elements at a time are taken from there, E > 1 only for rows on the grid.
+// One barrier a turn publishes the rows' sums, the next turn's data and the
+// stage to be filled again.
+//
+// HOLD: the turn's elements stay in registers across the barrier, as they
+// are stored, so its stage is filled again at once; else they are read again
+// and the stage is filled after the next barrier.  Two rows a turn share its
+// barrier, its waits and its shuffles: one row leaves a block of 16 warps,
+// all in step, with too little between them.
+struct NormGrad {
+  const void *g, *x, *w;
+  size_t g_stride, x_stride, dx_stride, rows;
+  const float2 *statistics;
+  void *dx;
+  float *partial;
+  unsigned cols, threads, slot;  // slot: bytes of one row in the ring
+};
+constexpr unsigned RING = 200 * 1024, DEPTH = 3, MAX_GROUPS = 15;  // named barriers 1 to 15
+
+// A thread's elements of one row as they are stored: WORDS registers.
+template <class T, int E, int K> struct Held {
+  static constexpr int N = K * E / 2;                       // pairs of elements
+  static constexpr int STEP = E == 1 ? 1 : E / 2;           // pairs of one access
+  static constexpr int WORDS = T::code == TC_F32 ? 2 * N : N;
+  uint32_t raw[WORDS];
+  __device__ __forceinline__ F2 pair_at(int i) const {
+    if constexpr (T::code == TC_F32) return pair(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
+    else return widen2<T>(raw[i]);
+  }
+  // The elements of `row` (in shared memory) at the columns of thread t;
+  // zeros past the row's end.
+  __device__ __forceinline__ void load(const typename T::S *row, unsigned t, unsigned threads, unsigned cols) {
+    using S = typename T::S;
+    if constexpr (E == 1) {
 #pragma unroll
-  for (int i = 0; i < K * E; ++i) sum_w[i] = sum_b[i] = 0.0f;
-  int turn = 0;
-  for (size_t r = blockIdx.x; r < rows; r += gridDim.x, turn ^= 1) {
-    Run<S, E> xr[K], gr[K];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const unsigned c = (t + k * threads) * E;
-      if (c < cols) {
-        xr[k] = load_run<S, E>(x + r * x_stride + c);
-        gr[k] = load_run<S, E>(g + r * g_stride + c);
+      for (int i = 0; i < N; ++i) {
+        const unsigned lo = t + 2 * i * threads, hi = lo + threads;
+        const S a = lo < cols ? row[lo] : S(0), b = hi < cols ? row[hi] : S(0);
+        if constexpr (T::code == TC_F32) {
+          raw[2 * i] = __float_as_uint(a);
+          raw[2 * i + 1] = __float_as_uint(b);
+        } else {
+          raw[i] = uint32_t(a) | uint32_t(b) << 16;
+        }
       }
-    }
-    const float2 st = statistics[r];
-    float s1 = 0.0f, s2 = 0.0f;
+    } else {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const unsigned c = (t + k * threads) * E;
-      if (c >= cols) break;
-      float wv[E];
-      if (w) load_wide<P, E>(w + c, wv);
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float h = (T::load(xr[k].e[j]) - st.x) * st.y, gv = T::load(gr[k].e[j]);
-        const float gw = w ? gv * wv[j] : gv;
-        s1 += gw;
-        s2 += gw * h;
-        sum_w[k * E + j] += gv * h;
-        sum_b[k * E + j] += gv;
+      for (int k = 0; k < K; ++k) {
+        const unsigned c = (t + k * threads) * E;
+        const uint4 v = c < cols ? *reinterpret_cast<const uint4 *>(row + c) : make_uint4(0, 0, 0, 0);
+        raw[4 * k] = v.x;
+        raw[4 * k + 1] = v.y;
+        raw[4 * k + 2] = v.z;
+        raw[4 * k + 3] = v.w;
       }
-    }
-    if (!dx) continue;
-    const float c1 = block_sum(s1, room[turn][0]) * share, c2 = block_sum(s2, room[turn][1]) * share;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const unsigned c = (t + k * threads) * E;
-      if (c >= cols) break;
-      float wv[E];
-      if (w) load_wide<P, E>(w + c, wv);
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float h = (T::load(xr[k].e[j]) - st.x) * st.y, gv = T::load(gr[k].e[j]);
-        xr[k].e[j] = T::store(st.y * ((w ? gv * wv[j] : gv) - c1 - h * c2));
-      }
-      store_run<S, E>(dx + r * dx_stride + c, xr[k]);
     }
   }
-  if (!partial) return;
-  float *pw = partial + size_t(blockIdx.x) * 2 * cols, *pb = pw + cols;
+};
+
+template <class T, class P, int E, int K, int R>
+__global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
+  using S = typename T::S;
+  using PS = typename P::S;
+  using Row = Held<T, E, K>;
+  constexpr int N = Row::N, STEP = Row::STEP;
+  constexpr bool HOLD = false, KEEP_W = K * E <= 16;
+  constexpr int GRANULES = K * E * int(sizeof(S)) / 16 + (E == 1);  // a thread's, of a row
+  extern __shared__ __align__(16) unsigned char ring[];
+  __shared__ float room[2][64];
+  const unsigned threads = a.threads, groups = blockDim.x / threads, cols = a.cols;
+  const unsigned group = threadIdx.x / threads, t = threadIdx.x - group * threads;
+  const unsigned lane = threadIdx.x & 31, warps = threads >> 5, warp0 = group * warps;
+  // turn n of this group: rows R (begin + n every), and the next
+  const size_t begin = size_t(blockIdx.x) * groups + group, every = size_t(gridDim.x) * groups;
+  const size_t turns = (a.rows + R - 1) / R, count = begin < turns ? (turns - begin + every - 1) / every : 0;
+  unsigned char *mine = ring + size_t(group) * DEPTH * 2 * R * a.slot;
+  const uint32_t mine32 = uint32_t(__cvta_generic_to_shared(mine));
+  auto column = [&](int k) { return (t + k * threads) * E; };
+  auto sync = [&] { __barrier_sync_count(group + 1, threads); };
+  auto row_at = [&](const void *p, size_t stride, size_t row) {
+    return reinterpret_cast<uintptr_t>(static_cast<const S *>(p) + row * stride);
+  };
+
+  // the next turn to be copied
+  size_t row_next = begin * R;
+  uintptr_t x_next = row_at(a.x, a.x_stride, row_next), g_next = row_at(a.g, a.g_stride, row_next);
+  const size_t x_step = a.x_stride * sizeof(S), g_step = a.g_stride * sizeof(S);
+  auto fetch = [&](uintptr_t from, uint32_t to) {
+    const unsigned off = E == 1 ? unsigned(from) & 15 : 0, bytes = off + cols * unsigned(sizeof(S));
+    const char *p = reinterpret_cast<const char *>(from - off) + t * 16;
+    to += t * 16;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const unsigned c = (t + k * threads) * E;
-    if (c >= cols) break;
+    for (int j = 0; j < GRANULES; ++j)
+      if ((t + j * threads) * 16 < bytes) copy_async(to + j * threads * 16, p + j * threads * 16);
+  };
+  auto fill = [&](unsigned stage) {
+    const uint32_t to = mine32 + stage * 2 * R * a.slot;
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      pw[c + j] = sum_w[k * E + j];
-      pb[c + j] = sum_b[k * E + j];
+    for (int r = 0; r < R; ++r)
+      if (row_next + r < a.rows) {
+        fetch(x_next + r * x_step, to + 2 * r * a.slot);
+        fetch(g_next + r * g_step, to + (2 * r + 1) * a.slot);
+      }
+    row_next += every * R;
+    x_next += every * R * x_step;
+    g_next += every * R * g_step;
+    copy_commit();
+  };
+  constexpr unsigned AHEAD = HOLD ? DEPTH : DEPTH - 1;  // turns in the ring at a turn's start
+#pragma unroll
+  for (unsigned d = 0; d < AHEAD; ++d) fill(d);
+
+  auto load_weight = [&](int i) -> F2 {  // pair i
+    if (!a.w) return pair(1.0f, 1.0f);
+    const PS *at = static_cast<const PS *>(a.w);
+    if constexpr (E == 1) {
+      const unsigned lo = column(2 * i), hi = column(2 * i + 1);
+      return pair(lo < cols ? P::load(at[lo]) : 1.0f, hi < cols ? P::load(at[hi]) : 1.0f);
+    } else {
+      const unsigned c = column(i / STEP) + i % STEP * 2;
+      if (c >= cols) return pair(1.0f, 1.0f);
+      const Run<PS, 2> r = load_run<PS, 2>(at + c);
+      return pair(P::load(r.e[0]), P::load(r.e[1]));
     }
+  };
+  F2 w[KEEP_W ? N : 1], sum_w[N], sum_b[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (KEEP_W) w[i] = load_weight(i);
+    sum_w[i] = sum_b[i] = 0;
+  }
+  auto weight = [&](int i) { return KEEP_W ? w[KEEP_W ? i : 0] : load_weight(i); };
+
+  const float share = 1.0f / float(cols);
+  size_t row = begin * R;
+  uintptr_t x_here = x_next - AHEAD * every * R * x_step, g_here = g_next - AHEAD * every * R * g_step;
+  S *dx = static_cast<S *>(a.dx) + (a.dx ? row * a.dx_stride : 0);
+  float2 next[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) next[r] = row + r < a.rows ? a.statistics[row + r] : make_float2(0.0f, 0.0f);
+  copy_wait<AHEAD - 1>();
+  sync();
+  unsigned stage = 0, turn = 0;
+  for (size_t n = 0; n < count; ++n, turn ^= 1) {
+    const unsigned char *here = mine + stage * 2 * R * a.slot;
+    auto held_at = [&](int which, uintptr_t from) {
+      return reinterpret_cast<const S *>(here + which * a.slot + (E == 1 ? from & 15 : 0));
+    };
+    Row xr[R], gr[R];
+    float2 st[R];
+    float value[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // sum(g w), sum(g w h) of each row
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      st[r] = next[r];
+      const bool real = R == 1 || row + r < a.rows;
+      // a row past the last has no data: no columns of it are read
+      xr[r].load(held_at(2 * r, x_here + r * x_step), t, threads, real ? cols : 0);
+      gr[r].load(held_at(2 * r + 1, g_here + r * g_step), t, threads, real ? cols : 0);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const F2 mean = pair(-st[r].x, -st[r].x), rstd = pair(st[r].y, st[r].y);
+      F2 s1 = 0, s2 = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const F2 h = mul2(add2(xr[r].pair_at(i), mean), rstd), gv = gr[r].pair_at(i), gw = mul2(gv, weight(i));
+        s1 = add2(s1, gw);
+        s2 = fma2(gw, h, s2);
+        sum_w[i] = fma2(gv, h, sum_w[i]);
+        sum_b[i] = add2(sum_b[i], gv);
+      }
+      const float2 p = split(s1), q = split(s2);
+      value[2 * r] = p.x + p.y;
+      value[2 * r + 1] = q.x + q.y;
+    }
+    // the warp's sums: each eighth of a warp's lanes ends with one of the four
+    const bool high = lane & 16, odd = lane & 8;
+    float v0 = high ? value[2] : value[0], v1 = high ? value[3] : value[1];
+    v0 += __shfl_xor_sync(0xffffffffu, high ? value[0] : value[2], 16);
+    v1 += __shfl_xor_sync(0xffffffffu, high ? value[1] : value[3], 16);
+    float v = odd ? v1 : v0;
+    v += __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 8);
+#pragma unroll
+    for (int o = 4; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    float *at = room[turn] + (lane >> 3) * 16;
+    if ((lane & 7) == 0) at[threadIdx.x >> 5] = v;
+    row += every * R;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (row + r < a.rows) next[r] = a.statistics[row + r];
+    copy_wait<AHEAD - 2>();  // this thread's part of the next turn
+    sync();
+    // every thread is past this turn's data (HOLD), or past the last turn's
+    fill(HOLD ? stage : stage == 0 ? DEPTH - 1 : stage - 1);
+    v = ((lane & 7) < warps ? at[warp0 + (lane & 7)] : 0.0f) + ((lane & 7) + 8 < warps ? at[warp0 + (lane & 7) + 8] : 0.0f);
+#pragma unroll
+    for (int o = 4; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    v *= -share;
+    if (a.dx) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float c1 = __shfl_sync(0xffffffffu, v, 16 * r) * st[r].y, c2 = __shfl_sync(0xffffffffu, v, 16 * r + 8) * st[r].y;
+        if (R > 1 && row - every * R + r >= a.rows) break;
+        const F2 mean = pair(-st[r].x, -st[r].x), rstd = pair(st[r].y, st[r].y), k1 = pair(c1, c1), k2 = pair(c2, c2);
+        if (!HOLD) {
+          xr[r].load(held_at(2 * r, x_here + r * x_step), t, threads, cols);
+          gr[r].load(held_at(2 * r + 1, g_here + r * g_step), t, threads, cols);
+        }
+#pragma unroll
+        for (int i = 0; i < N; i += STEP) {
+          F2 out[STEP];
+#pragma unroll
+          for (int j = 0; j < STEP; ++j) {
+            const F2 h = mul2(add2(xr[r].pair_at(i + j), mean), rstd), gw = mul2(gr[r].pair_at(i + j), weight(i + j));
+            out[j] = fma2(gw, rstd, fma2(h, k2, k1));
+          }
+          S *to = dx + r * a.dx_stride;
+          if constexpr (E == 1) {
+            const float2 o = split(out[0]);
+            const unsigned lo = column(2 * i), hi = column(2 * i + 1);
+            if (lo < cols) to[lo] = T::store(o.x);
+            if (hi < cols) to[hi] = T::store(o.y);
+          } else if (column(i / STEP) < cols) {
+            store_pairs<T>(to + column(i / STEP), out);
+          }
+        }
+      }
+      dx += every * R * a.dx_stride;
+    }
+    x_here += every * R * x_step;
+    g_here += every * R * g_step;
+    stage = stage + 1 == DEPTH ? 0 : stage + 1;
+  }
+  copy_wait<0>();
+  if (!a.partial) return;
+  // the groups' sums: each group's to the ring's memory, then added up in the
+  // groups' order by all threads
+  float *out = a.partial + size_t(blockIdx.x) * 2 * cols;
+  float *hold = groups > 1 ? reinterpret_cast<float *>(ring) + size_t(group) * 2 * cols : out;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float2 vw = split(sum_w[i]), vb = split(sum_b[i]);
+    const unsigned lo = E == 1 ? column(2 * i) : column(i / STEP) + i % STEP * 2, hi = E == 1 ? column(2 * i + 1) : lo + 1;
+    if (lo < cols) {
+      hold[lo] = vw.x;
+      hold[cols + lo] = vb.x;
+    }
+    if (hi < cols) {
+      hold[hi] = vw.y;
+      hold[cols + hi] = vb.y;
+    }
+  }
+  if (groups == 1) return;
+  __syncthreads();
+  hold = reinterpret_cast<float *>(ring);
+  for (unsigned c = threadIdx.x; c < 2 * cols; c += blockDim.x) {
+    float sum = hold[c];
+    for (unsigned g = 1; g < groups; ++g) sum += hold[size_t(g) * 2 * cols + c];
+    out[c] = sum;
   }
 }
 
@@ -382,23 +591,38 @@ int tc_layer_norm_backward(int dtype, int param_dtype, size_t rows, size_t cols,
                        runs_fit(x, x_stride, rows, sizeof(S), V) &&
                        (!grad_x || runs_fit(grad_x, grad_x_stride, rows, sizeof(S), V)) &&
                        (!weight || reinterpret_cast<uintptr_t>(weight) % 16 == 0);
-    auto launch = [&](auto e, auto k) -> int {
-      constexpr int E = decltype(e)::value, K = decltype(k)::value;
+    // Threads own 16 columns where 512 of them hold a row, else 32.  Two rows
+    // a turn where their registers and the ring hold them.
+    const bool narrow = cols <= 16 * 512;
+    const size_t slot = (std::min<size_t>(cols, 16 * 1024) * sizeof(S) + 15) / 16 * 16 + 16;
+    auto launch = [&](auto e, auto k, auto two) -> int {
+      constexpr int E = decltype(e)::value, K = decltype(k)::value, R = decltype(two)::value;
+      auto kernel = norm_grad_rows<T, P, E, K, R>;
+      static const cudaError_t allowed = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RING);
+      if (int st = check_cuda(allowed, "layer norm backward")) return st;
+      NormGrad a{grad, x, weight, grad_stride, x_stride, grad_x_stride, rows, stats, grad_x, nullptr, unsigned(cols), 0, unsigned(slot)};
       const unsigned n = unsigned((cols + E - 1) / E);
-      const unsigned threads = ((n + K - 1) / K + 31) / 32 * 32;
-      int resident = 0;
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, norm_grad_rows<T, P, E, K>, int(threads), 0);
-      const unsigned grid = unsigned(std::min<size_t>(rows, size_t(sm_count()) * size_t(std::max(1, resident))));
-      if (sums)
+      a.threads = ((n + K - 1) / K + 31) / 32 * 32;
+      // as many groups as the block's threads, its named barriers and the ring
+      // hold, but no more than give every SM a turn
+      const size_t sms = size_t(sm_count()), turns = (rows + R - 1) / R, each = DEPTH * 2 * R * slot;
+      const unsigned groups = unsigned(std::min<size_t>({MAX_GROUPS, 512 / a.threads, RING / each, (turns + sms - 1) / sms}));
+      const unsigned grid = unsigned(std::min<size_t>((turns + groups - 1) / groups, sms));
+      if (sums) {
         if (int st = room(grid)) return st;
-      norm_grad_rows<T, P, E, K><<<grid, threads, 0, on>>>(gs, grad_stride, xs, x_stride, stats, ws, dx, grad_x_stride,
-                                                           partial, rows, unsigned(cols));
+        a.partial = partial;
+      }
+      kernel<<<grid, groups * a.threads, std::max(groups * each, groups > 1 ? groups * cols * 8 : 0), on>>>(a);
       return check_launch("layer norm backward");
     };
-    if (cols <= 16 * 512) {
-      if (int st = whole ? launch(std::integral_constant<int, V>{}, std::integral_constant<int, 16 / V>{})
-                         : launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{}))
-        return st;
+    if (cols <= 16 * 1024 && DEPTH * 2 * slot <= RING) {
+      constexpr int R = sizeof(S) == 2 ? 2 : 1;
+      int st;
+      if (whole && narrow) st = launch(std::integral_constant<int, V>{}, std::integral_constant<int, 16 / V>{}, std::integral_constant<int, R>{});
+      else if (whole) st = launch(std::integral_constant<int, V>{}, std::integral_constant<int, 32 / V>{}, std::integral_constant<int, 1>{});
+      else if (narrow) st = launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+      else st = launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
+      if (st) return st;
     } else {
       if (sums) {  // first: grad_x may replace what they read
         const size_t tiles = (cols + 127) / 128;

@@ -37,6 +37,73 @@ template <class S, int E> __device__ __forceinline__ void store_run(S *p, const 
   *reinterpret_cast<W *>(p) = u.w;
 }
 
+// Two f32 in one register pair.  sm_100a adds, multiplies and fuses both in
+// one instruction, each half rounded as the scalar operation rounds it.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 pair(float lo, float hi) {
+  F2 p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+  return p;
+}
+__device__ __forceinline__ float2 split(F2 p) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+// A word of two elements of a 16-bit type, low first, widened and rounded as
+// the single ones are.
+template <class T> __device__ __forceinline__ F2 widen2(uint32_t w) {
+  if constexpr (T::code == TC_BF16) {
+    return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  } else {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    return pair(v.x, v.y);
+  }
+}
+template <class T> __device__ __forceinline__ uint32_t narrow2(F2 p) {
+  const float2 v = split(p);
+  if constexpr (T::code == TC_BF16) return pack2_bf16(v.x, v.y);
+  else return pack2_f16(v.x, v.y);
+}
+
+// E consecutive elements (16 bytes of them) as pairs of f32, and back.
+template <class T> __device__ __forceinline__ void load_pairs(const typename T::S *p, F2 *v) {
+  if constexpr (T::code == TC_F32) {
+    const ulonglong2 r = *reinterpret_cast<const ulonglong2 *>(p);
+    v[0] = r.x;
+    v[1] = r.y;
+  } else {
+    const uint4 r = *reinterpret_cast<const uint4 *>(p);
+    v[0] = widen2<T>(r.x);
+    v[1] = widen2<T>(r.y);
+    v[2] = widen2<T>(r.z);
+    v[3] = widen2<T>(r.w);
+  }
+}
+template <class T> __device__ __forceinline__ void store_pairs(typename T::S *p, const F2 *v) {
+  if constexpr (T::code == TC_F32) {
+    *reinterpret_cast<ulonglong2 *>(p) = make_ulonglong2(v[0], v[1]);
+  } else {
+    *reinterpret_cast<uint4 *>(p) = make_uint4(narrow2<T>(v[0]), narrow2<T>(v[1]), narrow2<T>(v[2]), narrow2<T>(v[3]));
+  }
+}
+
 // E consecutive elements of type T as f32, in accesses of at most 16 bytes.
 template <class T, int E> __device__ __forceinline__ void load_wide(const typename T::S *p, float (&v)[E]) {
   using S = typename T::S;
