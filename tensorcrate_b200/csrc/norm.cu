@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
     g_next += every * R * g_step;
     copy_commit();
   };
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr unsigned AHEAD = HOLD ? DEPTH : DEPTH - 1;  // turns in the ring at a turn's start
 #pragma unroll
   for (unsigned d = 0; d < AHEAD; ++d) fill(d);
@@ -450,29 +451,32 @@ __global__ void __launch_bounds__(128) norm_grad_columns(const typename T::S *g,
   partial[size_t(blockIdx.y) * 2 * cols + cols + c] = sb;
 }
 
-// grad_w and grad_b from the blocks' partial sums, added in the blocks'
-// order: 32 columns a block, its 8 warps each an eighth of the partials.
+// grad_w and grad_b from the blocks' partial sums, in an order that the sizes
+// give: 32 columns a block, each of its 32 warps a part of the partials.  The
+// block may be resident before the partials are written; it waits for them
+// where it says so.
 template <class P>
-__global__ void __launch_bounds__(256) norm_grad_join(const float *__restrict__ partial, unsigned parts, size_t cols,
-                                                      typename P::S *__restrict__ dw, typename P::S *__restrict__ db) {
-  __shared__ float room[8][33];
+__global__ void __launch_bounds__(1024) norm_grad_join(const float *partial, unsigned parts, size_t cols,
+                                                       typename P::S *__restrict__ dw, typename P::S *__restrict__ db) {
+  __shared__ float room[32][33];
   const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const size_t i = size_t(blockIdx.x) * 32 + lane;  // column of [w's sums | b's sums]
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   float v = 0.0f;
   if (i < 2 * cols) {
-#pragma unroll 8
-    for (unsigned p = warp; p < parts; p += 8) v += partial[size_t(p) * 2 * cols + i];
+#pragma unroll 5
+    for (unsigned p = warp; p < parts; p += 32) v += __ldcg(partial + size_t(p) * 2 * cols + i);
   }
   room[warp][lane] = v;
   __syncthreads();
-  if (warp || i >= 2 * cols) return;
-  float sum = 0.0f;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) sum += room[k][lane];
-  if (i < cols) {
-    if (dw) dw[i] = P::store(sum);
+  // warp w adds up column w of the block
+  const float sum = warp_sum(room[lane][warp]);
+  const size_t c = size_t(blockIdx.x) * 32 + warp;
+  if (lane || c >= 2 * cols) return;
+  if (c < cols) {
+    if (dw) dw[c] = P::store(sum);
   } else if (db) {
-    db[i - cols] = P::store(sum);
+    db[c - cols] = P::store(sum);
   }
 }
 
@@ -620,6 +624,7 @@ int tc_layer_norm_backward(int dtype, int param_dtype, size_t rows, size_t cols,
       int st;
       if (whole && narrow) st = launch(std::integral_constant<int, V>{}, std::integral_constant<int, 16 / V>{}, std::integral_constant<int, R>{});
       else if (whole) st = launch(std::integral_constant<int, V>{}, std::integral_constant<int, 32 / V>{}, std::integral_constant<int, 1>{});
+      else if (cols <= 8 * 512) st = launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
       else if (narrow) st = launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
       else st = launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
       if (st) return st;
@@ -639,8 +644,18 @@ int tc_layer_norm_backward(int dtype, int param_dtype, size_t rows, size_t cols,
       }
     }
     if (!sums) return TC_OK;
-    const size_t blocks = (2 * cols + 31) / 32;
-    norm_grad_join<P><<<unsigned(blocks), 256, 0, on>>>(partial, parts, cols, dw, db);
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(unsigned((2 * cols + 31) / 32));
+    config.blockDim = dim3(1024);
+    config.stream = on;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    if (int st = check_cuda(cudaLaunchKernelEx(&config, norm_grad_join<P>, static_cast<const float *>(partial), parts, cols, dw, db),
+                            "layer norm backward"))
+      return st;
     return check_launch("layer norm backward");
   });
 }
