@@ -13,6 +13,7 @@
 // and the gradient 0.  A NaN or an infinity among a row's logits makes the
 // row's results NaN, as the formulas do.  The reference has no counterpart.
 #include <algorithm>
+#include <type_traits>
 
 #include "rows.cuh"
 
@@ -20,15 +21,16 @@ namespace tc {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-__device__ __forceinline__ float exp_of(float x) {
+__device__ __forceinline__ float exp2_of(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * LOG2E));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float exp_of(float x) { return exp2_of(x * LOG2E); }
 
-// The running statistics of some elements of a row: their maximum (NaNs
-// passed over), the sum of exp(x - m) and, for the entropy, the sum of
-// exp(x - m) (x - m).  While m is -inf the sums are those of exp(x).
+// The statistics of some elements of a row: their maximum (NaNs passed
+// over), the sum of exp(x - m) and, for the entropy, the sum of exp(x - m)
+// (x - m).  While m is -inf the sums are those of exp(x).
 struct Sums {
   float m = -INFINITY, s = 0.0f, t = 0.0f;
 };
@@ -36,14 +38,12 @@ __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f
 
 // Restate the sums for the larger maximum `m`.
 template <bool ENT> __device__ __forceinline__ void raise(Sums &a, float m) {
-  if (a.m == -INFINITY) {  // s and t are 0, or NaN
-    a.m = m;
-    return;
+  if (a.m != -INFINITY) {  // else s and t are 0, or NaN
+    // the bound keeps up s finite where a.m is as low as the type goes (f is 0)
+    const float up = fminf(m - a.m, 1e20f), f = exp_of(-up);
+    if (ENT) a.t = f * (a.t - up * a.s);
+    a.s *= f;
   }
-  // the bound keeps up s finite where a.m is as low as the type goes (f is 0)
-  const float up = fminf(m - a.m, 1e20f), f = exp_of(-up);
-  if (ENT) a.t = f * (a.t - up * a.s);
-  a.s *= f;
   a.m = m;
 }
 template <bool ENT> __device__ __forceinline__ void join(Sums &a, Sums b) {
@@ -52,65 +52,130 @@ template <bool ENT> __device__ __forceinline__ void join(Sums &a, Sums b) {
   a.s += b.s;
   if (ENT) a.t += b.t;
 }
-template <bool ENT, int E> __device__ __forceinline__ void push(Sums &a, const float (&v)[E]) {
-  const float base = base_of(a.m);
+// Over a warp: the maximum first, so that each lane restates its sums once.
+template <bool ENT> __device__ __forceinline__ Sums warp_join(Sums a) {
+  float m = a.m;
 #pragma unroll
-  for (int j = 0; j < E; ++j) {
-    const float d = v[j] - base, e = exp_of(d);
-    a.s += e;
-    if (ENT) a.t += e * fmaxf(d, -1e30f);  // 0 for an element of -inf, NaN for a NaN (e is one)
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (m > a.m) raise<ENT>(a, m);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    if (ENT) a.t += __shfl_xor_sync(0xffffffffu, a.t, o);
   }
+  return a;
 }
 template <bool ENT> __device__ __forceinline__ Sums block_join(Sums a, Sums *room) {
-  auto across = [](Sums v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      Sums b;
-      b.m = __shfl_xor_sync(0xffffffffu, v.m, o);
-      b.s = __shfl_xor_sync(0xffffffffu, v.s, o);
-      if (ENT) b.t = __shfl_xor_sync(0xffffffffu, v.t, o);
-      join<ENT>(v, b);
-    }
-    return v;
-  };
-  a = across(a);
+  a = warp_join<ENT>(a);
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   if (lane == 0) room[threadIdx.x >> 5] = a;
   __syncthreads();
-  return across(lane < warps ? room[lane] : Sums{});
+  return warp_join<ENT>(lane < warps ? room[lane] : Sums{});
 }
 
-// A row's elements as runs of 16 aligned bytes, with the few before and
-// after them.
-template <class S> struct Cut {
-  static constexpr unsigned V = 16 / sizeof(S);
-  unsigned head, runs, tail, after;  // `tail` elements from `after`
-  __device__ __forceinline__ Cut(const S *row, unsigned n) {
-    const unsigned off = unsigned(reinterpret_cast<uintptr_t>(row) & 15) / unsigned(sizeof(S));
-    head = min(n, (V - off) % V);
-    runs = (n - head) / V;
-    after = head + runs * V;
-    tail = n - after;
+// 16 bytes of a row: V elements, as they are stored.
+template <class T> struct Bits {
+  static constexpr unsigned V = 16 / sizeof(typename T::S), PAIRS = V / 2;
+  uint4 w;
+  __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
+  __device__ __forceinline__ F2 pair_at(int i) const {
+    if constexpr (T::code == TC_F32) return pair(__uint_as_float(word(2 * i)), __uint_as_float(word(2 * i + 1)));
+    else return widen2<T>(word(i));
+  }
+  // The element, widened, with an index known at run time.
+  __device__ __forceinline__ float at(unsigned i) const {
+    if constexpr (T::code == TC_F32) return __uint_as_float(word(i));
+    else return T::load(uint16_t(word(i / 2) >> (i % 2 * 16)));
+  }
+};
+// The largest of the elements of U of them, NaNs passed over.
+template <class T, int U> __device__ __forceinline__ float largest(const Bits<T> (&r)[U]) {
+  if constexpr (T::code == TC_F32) {
+    float m = r[0].at(0);
+#pragma unroll
+    for (int i = 1; i < 4 * U; ++i) m = fmaxf(m, __uint_as_float(r[i / 4].word(i % 4)));
+    return m;
+  } else {
+    using H2 = std::conditional_t<T::code == TC_BF16, __nv_bfloat162, __half2>;
+    auto as = [](uint32_t w) { return *reinterpret_cast<const H2 *>(&w); };
+    H2 m = as(r[0].word(0));
+#pragma unroll
+    for (int i = 1; i < 4 * U; ++i) m = __hmax2(m, as(r[i / 4].word(i % 4)));
+    const float2 v = split(widen2<T>(*reinterpret_cast<const uint32_t *>(&m)));
+    return fmaxf(v.x, v.y);
+  }
+}
+
+// A thread's statistics while it walks, the sums in two halves.
+template <class T, bool ENT> struct Running {
+  float m = -INFINITY, base = 0.0f;
+  F2 s = 0, t = 0;
+  __device__ __forceinline__ void lift(float to) {
+    if (m != -INFINITY) {
+      const float up = fminf(to - m, 1e20f), f = exp_of(-up);
+      if (ENT) t = mul2(pair(f, f), fma2(pair(-up, -up), s, t));
+      s = mul2(pair(f, f), s);
+    }
+    m = base = to;
+  }
+  // Add a pair whose elements m is not below.
+  __device__ __forceinline__ void add(F2 v) {
+    const F2 d = add2(v, pair(-base, -base));
+    const float2 x = split(mul2(d, pair(LOG2E, LOG2E)));
+    const F2 e = pair(exp2_of(x.x), exp2_of(x.y));
+    s = add2(s, e);
+    if (ENT) {
+      // 0 for an element of -inf, NaN for a NaN (e is one)
+      const float2 y = split(d);
+      t = fma2(e, pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), t);
+    }
+  }
+  __device__ __forceinline__ Sums sums() const {
+    const float2 a = split(s), b = split(t);
+    return Sums{m, a.x + a.y, b.x + b.y};
   }
 };
 
-// one(index, value) for the single elements of a row that thread t of
-// `threads` takes, many(index, run) for its runs, in ascending order.
-template <class S, class One, class Many>
-__device__ __forceinline__ void walk(const S *row, const Cut<S> &c, unsigned t, unsigned threads, One &&one, Many &&many) {
-  constexpr unsigned V = Cut<S>::V;
+// A row's elements, or the part of them that one of `of` blocks has, as runs
+// of 16 aligned bytes with the few single elements before and after them.
+template <class T> struct Cut {
+  using S = typename T::S;
+  static constexpr unsigned V = 16 / sizeof(S);
+  unsigned head, body, runs, after, tail;  // [0, head), runs from body, `tail` from after
+  __device__ __forceinline__ Cut(const S *row, unsigned n, unsigned part = 0, unsigned of = 1) {
+    const unsigned off = unsigned(reinterpret_cast<uintptr_t>(row) & 15) / unsigned(sizeof(S));
+    head = min(n, (V - off) % V);
+    const unsigned all = (n - head) / V, from = unsigned((unsigned long long)all * part / of);
+    body = head + from * V;
+    runs = unsigned((unsigned long long)all * (part + 1) / of) - from;
+    after = head + all * V;
+    tail = part + 1 == of ? n - after : 0;
+    if (part) head = 0;
+  }
+};
+
+// one(index, value) for the single elements that thread t of `threads` takes,
+// many(index, bits, runs apart) for its runs, up to four at once, in ascending order.
+template <class T, class Load, class One, class Many>
+__device__ __forceinline__ void walk(const typename T::S *row, const Cut<T> &c, unsigned t, unsigned threads, Load &&load,
+                                     One &&one, Many &&many) {
   if (t < c.head) one(t, row[t]);
-  const S *body = row + c.head;
   unsigned i = t;
   for (; c.runs > 3 * threads && i < c.runs - 3 * threads; i += 4 * threads) {
-    Run<S, V> r[4];
+    Bits<T> r[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) r[u] = load_run<S, V>(body + size_t(i + u * threads) * V);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) many(c.head + (i + u * threads) * V, r[u]);
+    for (int u = 0; u < 4; ++u) r[u] = load(i + u * threads);
+    many(i, r);
   }
-  for (; i < c.runs; i += threads) many(c.head + i * V, load_run<S, V>(body + size_t(i) * V));
+  for (; i < c.runs; i += threads) {
+    Bits<T> r[1] = {load(i)};
+    many(i, r);
+  }
   if (t < c.tail) one(c.after + t, row[c.after + t]);
+}
+template <class T> __device__ __forceinline__ auto from_row(const typename T::S *row, const Cut<T> &c) {
+  const uint4 *p = reinterpret_cast<const uint4 *>(row + c.body);
+  return [p](unsigned i) { return Bits<T>{p[i]}; };
 }
 
 // ---------------------------------------------------------------------------
@@ -144,10 +209,11 @@ struct TopRoom {
 // them.  Those threads' elements are read again, the ones that reach the
 // bound are kept and ranked by counting.
 template <class T>
-__device__ __forceinline__ void top_of_row(const typename T::S *row, const Cut<typename T::S> &c, Key mine, float m,
-                                           unsigned k, TopRoom &room) {
+__device__ __forceinline__ void top_of_row(const typename T::S *row, const Cut<T> &c, Key mine, float m, unsigned k,
+                                           TopRoom &room) {
   using S = typename T::S;
-  constexpr unsigned V = Cut<S>::V;
+  constexpr unsigned V = Cut<T>::V;
+  const auto load = from_row<T>(row, c);
   const unsigned t = threadIdx.x, threads = blockDim.x, lanes = threads / GROUPS;
   Key g = mine;
   for (unsigned o = 1; o < lanes; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
@@ -174,9 +240,9 @@ __device__ __forceinline__ void top_of_row(const typename T::S *row, const Cut<t
   __syncthreads();
   for (unsigned h = t >> 5; h < room.holders; h += threads >> 5)
     for (size_t i = room.holder[h] + size_t(t & 31) * threads; i < c.runs; i += size_t(threads) * 32) {
-      const Run<S, V> r = load_run<S, V>(row + c.head + i * V);
+      const Bits<T> r = load(unsigned(i));
 #pragma unroll
-      for (unsigned j = 0; j < V; ++j) keep(c.head + unsigned(i) * V + j, T::load(r.e[j]));
+      for (unsigned j = 0; j < V; ++j) keep(c.body + unsigned(i) * V + j, r.at(j));
     }
   __syncthreads();
   const unsigned count = room.count;
@@ -195,14 +261,18 @@ __device__ __forceinline__ void top_of_row(const typename T::S *row, const Cut<t
   Key last = ~Key(0);
   for (unsigned n = 0; n < k; ++n) {
     Key best = 0;
-    auto one = [&](unsigned at, S e) {
-      const Key key = key_of(T::load(e), at);
+    auto each = [&](unsigned at, float v) {
+      const Key key = key_of(v, at);
       if (key < last && key > best) best = key;
     };
-    walk(row, c, t, threads, one, [&](unsigned at, const Run<S, V> &r) {
+    auto many = [&](unsigned i, const auto &r) {
+      constexpr int U = sizeof(r) / sizeof(r[0]);
 #pragma unroll
-      for (unsigned j = 0; j < V; ++j) one(at + j, r.e[j]);
-    });
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (unsigned j = 0; j < V; ++j) each(c.body + (i + u * threads) * V + j, r[u].at(j));
+    };
+    walk<T>(row, c, t, threads, load, [&](unsigned at, S e) { each(at, T::load(e)); }, many);
 #pragma unroll
     for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
     if ((t & 31) == 0) room.group[t >> 5] = best;
@@ -229,36 +299,72 @@ template <bool ENT> __device__ __forceinline__ float slope_at(const Slope &g, fl
   if (ENT) d -= g.v * p * (fmaxf(a, -1e30f) + g.entropy);
   return d;
 }
-template <class T, bool ENT>
-__device__ __forceinline__ void write_slope(const typename T::S *row, typename T::S *to, const Cut<typename T::S> &c,
-                                            const Slope &g, unsigned t, unsigned threads) {
+template <bool ENT> __device__ __forceinline__ F2 slope_of_pair(const Slope &g, F2 x) {
+  const F2 a = add2(add2(x, pair(-g.base, -g.base)), pair(-g.log_sum, -g.log_sum));
+  const float2 y = split(mul2(a, pair(LOG2E, LOG2E)));
+  const F2 p = pair(exp2_of(y.x), exp2_of(y.y));
+  if (!ENT) return mul2(p, pair(-g.u, -g.u));
+  // -p (u + v (a + H))
+  const float2 z = split(a);
+  const F2 c = add2(pair(fmaxf(z.x, -1e30f), fmaxf(z.y, -1e30f)), pair(g.entropy, g.entropy));
+  return mul2(p, fma2(c, pair(-g.v, -g.v), pair(-g.u, -g.u)));
+}
+// load(i) gives the row's run i; elements before and after the runs, and the
+// token's, are read from the row.
+template <class T, bool ENT, class Load>
+__device__ __forceinline__ void write_slope(const typename T::S *row, typename T::S *to, const Cut<T> &c, const Slope &g,
+                                            unsigned t, unsigned threads, Load &&load) {
   using S = typename T::S;
-  constexpr unsigned V = Cut<S>::V;
+  constexpr unsigned V = Cut<T>::V;
   const bool whole = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(to)) & 15) == 0;
+  auto put = [&](unsigned at, uint4 w) {
+    if (whole) {
+      *reinterpret_cast<uint4 *>(to + at) = w;
+    } else {
+      union {
+        uint4 w;
+        S e[V];
+      } u;
+      u.w = w;
+#pragma unroll
+      for (unsigned j = 0; j < V; ++j) to[at + j] = u.e[j];
+    }
+  };
   if (g.u == 0.0f && (!ENT || g.v == 0.0f)) {
     // nothing flows back through this row, whatever its logits
-    const Run<S, V> zero{};
     if (t < c.head) to[t] = S(0);
-    for (unsigned i = t; i < c.runs; i += threads) {
-      S *at = to + c.head + size_t(i) * V;
-      if (whole) store_run<S, V>(at, zero);
-      else
-#pragma unroll
-        for (unsigned j = 0; j < V; ++j) at[j] = S(0);
-    }
+    for (unsigned i = t; i < c.runs; i += threads) put(c.body + i * V, make_uint4(0, 0, 0, 0));
     if (t < c.tail) to[c.after + t] = S(0);
     return;
   }
-  walk(
-      row, c, t, threads, [&](unsigned at, S e) { to[at] = T::store(slope_at<ENT>(g, T::load(e), at)); },
-      [&](unsigned at, Run<S, V> r) {
+  auto many = [&](unsigned i, const auto &r) {
+    constexpr int U = sizeof(r) / sizeof(r[0]);
 #pragma unroll
-        for (unsigned j = 0; j < V; ++j) r.e[j] = T::store(slope_at<ENT>(g, T::load(r.e[j]), at + j));
-        if (whole) store_run<S, V>(to + at, r);
-        else
+    for (int u = 0; u < U; ++u) {
+      const unsigned at = c.body + (i + u * threads) * V;
+      F2 d[V / 2];
 #pragma unroll
-          for (unsigned j = 0; j < V; ++j) to[at + j] = r.e[j];
-      });
+      for (unsigned j = 0; j < V / 2; ++j) d[j] = slope_of_pair<ENT>(g, r[u].pair_at(j));
+      union {
+        uint4 w;
+        S e[V];
+      } out;
+      if constexpr (T::code == TC_F32) {
+        const float2 lo = split(d[0]), hi = split(d[1]);
+        out.w = make_uint4(__float_as_uint(lo.x), __float_as_uint(lo.y), __float_as_uint(hi.x), __float_as_uint(hi.y));
+      } else {
+        out.w = make_uint4(narrow2<T>(d[0]), narrow2<T>(d[1]), narrow2<T>(d[2]), narrow2<T>(d[3]));
+      }
+      if (g.token - at < V) {
+        const S special = T::store(slope_at<ENT>(g, r[u].at(g.token - at), g.token));
+#pragma unroll
+        for (unsigned j = 0; j < V; ++j)
+          if (at + j == g.token) out.e[j] = special;
+      }
+      put(at, out.w);
+    }
+  };
+  walk<T>(row, c, t, threads, load, [&](unsigned at, S e) { to[at] = T::store(slope_at<ENT>(g, T::load(e), at)); }, many);
 }
 
 struct TokenArgs {
@@ -295,44 +401,45 @@ enum Extra { NOTHING = 0, TOP = 1, GRADIENT = 2 };
 // A block a row: the statistics in one pass, and then what is asked for.
 template <class T, bool ENT, int EXTRA> __global__ void __launch_bounds__(512) token_rows(TokenArgs a) {
   using S = typename T::S;
-  constexpr unsigned V = Cut<S>::V;
+  constexpr unsigned V = Cut<T>::V;
   __shared__ Sums room[16];
   const unsigned t = threadIdx.x, threads = blockDim.x;
   for (size_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const S *row = static_cast<const S *>(a.logits) + r * a.stride;
-    const Cut<S> c(row, a.vocab);
+    const Cut<T> c(row, a.vocab);
     const unsigned token = a.tokens ? a.tokens[r] : ~0u;
     const float at_token = token < a.vocab ? T::load(row[token]) : __int_as_float(0x7fc00000);
-    Sums sums;
+    Running<T, ENT> run;
     // where the thread's largest element lies; its first, while all are -inf
-    unsigned at = t < c.head ? t : t < c.runs ? c.head + t * V : t < c.tail ? c.after + t : ~0u;
-    walk(
-        row, c, t, threads,
-        [&](unsigned i, S e) {
-          const float v[1] = {T::load(e)};
-          if (v[0] > sums.m) {
-            raise<ENT>(sums, v[0]);
-            if (EXTRA == TOP) at = i;
-          }
-          push<ENT, 1>(sums, v);
-        },
-        [&](unsigned i, const Run<S, V> &run) {
-          float v[V];
+    unsigned at = t < c.head ? t : t < c.runs ? c.body + t * V : t < c.tail ? c.after + t : ~0u;
+    auto one = [&](unsigned i, S e) {
+      const float v = T::load(e);
+      if (v > run.m) {
+        run.lift(v);
+        if (EXTRA == TOP) at = i;
+      }
+      run.add(pair(v, -INFINITY));
+    };
+    auto many = [&](unsigned i, const auto &bits) {
+      constexpr int U = sizeof(bits) / sizeof(bits[0]);
+      const float m = largest(bits);
+      if (m > run.m) {
+        run.lift(m);
+        if (EXTRA == TOP) {
 #pragma unroll
-          for (unsigned j = 0; j < V; ++j) v[j] = T::load(run.e[j]);
-          float m = v[0];
+          for (int u = U - 1; u >= 0; --u)
 #pragma unroll
-          for (unsigned j = 1; j < V; ++j) m = fmaxf(m, v[j]);
-          if (m > sums.m) {
-            raise<ENT>(sums, m);
-            if (EXTRA == TOP) {
+            for (int j = int(V) - 1; j >= 0; --j)
+              if (bits[u].at(j) == m) at = c.body + (i + u * threads) * V + unsigned(j);
+        }
+      }
 #pragma unroll
-              for (int j = int(V) - 1; j >= 0; --j)
-                if (v[j] == m) at = i + unsigned(j);
-            }
-          }
-          push<ENT, V>(sums, v);
-        });
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (unsigned j = 0; j < V / 2; ++j) run.add(bits[u].pair_at(j));
+    };
+    walk<T>(row, c, t, threads, from_row<T>(row, c), one, many);
+    const Sums sums = run.sums();
     const Sums all = block_join<ENT>(sums, room);
     const bool empty = all.m == -INFINITY && all.s == 0.0f;
     const float2 st = make_float2(all.m, empty ? 0.0f : logf(all.s));
@@ -354,7 +461,7 @@ template <class T, bool ENT, int EXTRA> __global__ void __launch_bounds__(512) t
       }
     }
     if (EXTRA == GRADIENT)
-      write_slope<T, ENT>(row, static_cast<S *>(a.grad_logits) + r * a.grad_stride, c, slope_of(a, r, st, entropy), t, threads);
+      write_slope<T, ENT>(row, static_cast<S *>(a.grad_logits) + r * a.grad_stride, c, slope_of(a, r, st, entropy), t, threads, from_row<T>(row, c));
     __syncthreads();
   }
 }
@@ -364,9 +471,10 @@ template <class T, bool ENT> __global__ void __launch_bounds__(512) token_slope(
   using S = typename T::S;
   for (size_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const S *row = static_cast<const S *>(a.logits) + r * a.stride;
-    const Cut<S> c(row, a.vocab);
+    const Cut<T> c(row, a.vocab);
     write_slope<T, ENT>(row, static_cast<S *>(a.grad_logits) + r * a.grad_stride, c,
-                        slope_of(a, r, a.kept_statistics[r], ENT ? a.kept_entropy[r] : 0.0f), threadIdx.x, blockDim.x);
+                        slope_of(a, r, a.kept_statistics[r], ENT ? a.kept_entropy[r] : 0.0f), threadIdx.x, blockDim.x,
+                        from_row<T>(row, c));
   }
 }
 
