@@ -65,14 +65,6 @@ template <bool ENT> __device__ __forceinline__ Sums warp_join(Sums a) {
   }
   return a;
 }
-template <bool ENT> __device__ __forceinline__ Sums block_join(Sums a, Sums *room) {
-  a = warp_join<ENT>(a);
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  if (lane == 0) room[threadIdx.x >> 5] = a;
-  __syncthreads();
-  return warp_join<ENT>(lane < warps ? room[lane] : Sums{});
-}
-
 // 16 bytes of a row: V elements, as they are stored.
 template <class T> struct Bits {
   static constexpr unsigned V = 16 / sizeof(typename T::S), PAIRS = V / 2;
@@ -106,37 +98,121 @@ template <class T, int U> __device__ __forceinline__ float largest(const Bits<T>
   }
 }
 
-// A thread's statistics while it walks, the sums in two halves.
-template <class T, bool ENT> struct Running {
-  float m = -INFINITY, base = 0.0f;
-  F2 s = 0, t = 0;
-  __device__ __forceinline__ void lift(float to) {
-    if (m != -INFINITY) {
-      const float up = fminf(to - m, 1e20f), f = exp_of(-up);
-      if (ENT) t = mul2(pair(f, f), fma2(pair(-up, -up), s, t));
-      s = mul2(pair(f, f), s);
-    }
-    m = base = to;
+// From here on a logit's weight is e = 2^a, a = x log2(e) - mark: one fused
+// operation.  The mark is m log2(e) rounded, which shifts every a of a row by
+// the same amount, known exactly, and is undone in what is taken from the
+// sums.  That holds for |m| up to TAME, where the shift is below 2^-13; past
+// it (a row masked by the type's lowest value, say) a = (x - m) log2(e), the
+// difference first.
+constexpr float TAME = 1024.0f, LN2 = 0.6931471805599453f;
+__device__ __forceinline__ bool tame(float m) { return fabsf(m) <= TAME; }
+
+// A pair of elements no lower than -1e37 (-65504): weightless wherever m is
+// tame, and finite.  NaNs stay.
+template <class T> __device__ __forceinline__ Bits<T> lifted(Bits<T> r) {
+  if constexpr (T::code == TC_F32) {
+    auto up = [](uint32_t w) {
+      float v;
+      asm("max.NaN.f32 %0, %1, 0fFCF0BDC2;" : "=f"(v) : "f"(__uint_as_float(w)));  // -1e37
+      return __float_as_uint(v);
+    };
+    return Bits<T>{make_uint4(up(r.w.x), up(r.w.y), up(r.w.z), up(r.w.w))};
+  } else {
+    auto up = [](uint32_t w) {
+      uint32_t v;
+      if constexpr (T::code == TC_BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(v) : "r"(w), "r"(0xfcf0fcf0u));
+      else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(v) : "r"(w), "r"(0xfbfffbffu));
+      return v;
+    };
+    return Bits<T>{make_uint4(up(r.w.x), up(r.w.y), up(r.w.z), up(r.w.w))};
   }
-  // Add a pair whose elements m is not below.
-  __device__ __forceinline__ void add(F2 v) {
-    const F2 d = add2(v, pair(-base, -base));
-    const float2 x = split(mul2(d, pair(LOG2E, LOG2E)));
+}
+
+// A thread's statistics while it walks: the maximum, and the sums of e and of
+// e a, each in two halves.  The mark is that of an earlier maximum as long as
+// the present one is within 8 of it (e is then below 2^12): few marks change,
+// where among 32 lanes some maximum does all the time.
+template <class T, bool ENT> struct Running {
+  float m = -INFINITY, ref = -INFINITY, limit = -INFINITY, mark = 0.0f;
+  bool wild = false;
+  F2 s = 0, t = 0;
+  __device__ __forceinline__ void begin(float at) {
+    m = ref = at;
+    wild = !tame(at) && at != -INFINITY;
+    mark = at == -INFINITY || wild ? 0.0f : at * LOG2E;
+    limit = at == -INFINITY || wild ? at : at + 8.0f;
+  }
+  __device__ __forceinline__ void lift(float to) {
+    const Running old = *this;
+    begin(to);
+    if (old.ref == -INFINITY) return;
+    const float up = old.wild || wild ? fminf((to - old.ref) * LOG2E, 1e20f) : mark - old.mark, f = exp2_of(-up);
+    if (ENT) t = mul2(pair(f, f), fma2(pair(-up, -up), s, t));
+    s = mul2(pair(f, f), s);
+  }
+  __device__ __forceinline__ void weigh(F2 a) {
+    const float2 x = split(a);
     const F2 e = pair(exp2_of(x.x), exp2_of(x.y));
     s = add2(s, e);
-    if (ENT) {
-      // 0 for an element of -inf, NaN for a NaN (e is one)
-      const float2 y = split(d);
-      t = fma2(e, pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), t);
+    if (ENT) t = fma2(e, a, t);
+  }
+  // Elements that m is not below.
+  template <int U> __device__ __forceinline__ void add(const Bits<T> (&r)[U]) {
+    if (wild) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < int(Bits<T>::PAIRS); ++j) add_wild(r[u].pair_at(j));
+      return;
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const Bits<T> b = ENT ? lifted(r[u]) : r[u];
+#pragma unroll
+      for (int j = 0; j < int(Bits<T>::PAIRS); ++j) weigh(fma2(b.pair_at(j), pair(LOG2E, LOG2E), pair(-mark, -mark)));
+    }
+  }
+  __device__ __forceinline__ void add_wild(F2 v) {
+    const float2 d = split(add2(v, pair(-base_of(ref), -base_of(ref))));
+    const float2 e = make_float2(exp_of(d.x), exp_of(d.y));
+    s = add2(s, pair(e.x, e.y));
+    // 0 for an element of -inf, NaN for a NaN (e is one)
+    if (ENT) t = fma2(pair(e.x, e.y), pair(fmaxf(d.x * LOG2E, -1e30f), fmaxf(d.y * LOG2E, -1e30f)), t);
+  }
+  __device__ __forceinline__ void add_one(float v) {
+    if (wild || ref == -INFINITY) {
+      add_wild(pair(v, -INFINITY));
+      return;
+    }
+    const float a = fmaf(v, LOG2E, -mark), e = exp2_of(a);
+    s = add2(s, pair(e, 0.0f));
+    if (ENT) t = add2(t, pair(e * fmaxf(a, -1e30f), 0.0f));
+  }
+  // True where they raised the maximum.
+  template <int U> __device__ __forceinline__ bool take(const Bits<T> (&r)[U]) {
+    const float top = largest(r);
+    const bool more = top > m;
+    if (top > limit) lift(top);
+    m = fmaxf(m, top);
+    add(r);
+    return more;
+  }
+  __device__ __forceinline__ bool take_one(float v) {
+    const bool more = v > m;
+    if (v > limit) lift(v);
+    m = fmaxf(m, v);
+    add_one(v);
+    return more;
   }
   __device__ __forceinline__ Sums sums() const {
     const float2 a = split(s), b = split(t);
-    return Sums{m, a.x + a.y, b.x + b.y};
+    const float off = wild || m == -INFINITY ? 0.0f : fmaf(m, LOG2E, -mark), f = exp2_of(-off), sum = a.x + a.y;
+    return Sums{m, sum * f, (b.x + b.y - off * sum) * (f * LN2)};
   }
 };
 
-// A row's elements, or the part of them that one of `of` blocks has, as runs
+// A row's elements, or the part of them that one of `of` (a power of two)
+// blocks has, as runs
 // of 16 aligned bytes with the few single elements before and after them.
 template <class T> struct Cut {
   using S = typename T::S;
@@ -145,9 +221,9 @@ template <class T> struct Cut {
   __device__ __forceinline__ Cut(const S *row, unsigned n, unsigned part = 0, unsigned of = 1) {
     const unsigned off = unsigned(reinterpret_cast<uintptr_t>(row) & 15) / unsigned(sizeof(S));
     head = min(n, (V - off) % V);
-    const unsigned all = (n - head) / V, from = unsigned((unsigned long long)all * part / of);
+    const unsigned all = (n - head) / V, per = (all + of - 1) >> (31 - __clz(of)), from = min(all, part * per);
     body = head + from * V;
-    runs = unsigned((unsigned long long)all * (part + 1) / of) - from;
+    runs = min(all - from, per);
     after = head + all * V;
     tail = part + 1 == of ? n - after : 0;
     if (part) head = 0;
@@ -155,7 +231,8 @@ template <class T> struct Cut {
 };
 
 // one(index, value) for the single elements that thread t of `threads` takes,
-// many(index, bits, runs apart) for its runs, up to four at once, in ascending order.
+// many(first run, bits) for its runs (`threads` apart), up to four at once, in
+// ascending order.
 template <class T, class Load, class One, class Many>
 __device__ __forceinline__ void walk(const typename T::S *row, const Cut<T> &c, unsigned t, unsigned threads, Load &&load,
                                      One &&one, Many &&many) {
@@ -178,6 +255,56 @@ template <class T> __device__ __forceinline__ auto from_row(const typename T::S 
   return [p](unsigned i) { return Bits<T>{p[i]}; };
 }
 
+// The blocks of a cluster share a row: this block's part, and how many there
+// are (1 without a cluster).
+__device__ __forceinline__ unsigned cluster_part() {
+  unsigned v;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(v));
+  return v;
+}
+__device__ __forceinline__ unsigned cluster_parts() {
+  unsigned v;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(v));
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Store to the same variable of block `part`.
+template <class V> __device__ __forceinline__ void store_at(V *own, unsigned part, V v) {
+  uint32_t to;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(uint32_t(__cvta_generic_to_shared(own))), "r"(part));
+  if constexpr (sizeof(V) == 4) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(__float_as_uint(v)) : "memory");
+  else asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(to), "l"(v) : "memory");
+}
+// The sums of a row over the warps of the cluster's blocks (at most 64), the
+// same in every thread: each warp's go to every block.  The slots of two rows
+// in turn: a warp that is ahead stores a row's sums while another still reads
+// the last row's.
+struct Slots {
+  Sums of[2][64];
+};
+template <bool ENT> __device__ __forceinline__ Sums row_join(Sums mine, Slots &slots, unsigned part, unsigned parts, unsigned turn) {
+  const unsigned lane = threadIdx.x & 31, warps = blockDim.x >> 5, n = parts * warps;
+  Sums *all = slots.of[turn];
+  mine = warp_join<ENT>(mine);
+  if (parts == 1) {
+    if (lane == 0) all[threadIdx.x >> 5] = mine;
+    __syncthreads();
+  } else {
+    if (lane < parts) {
+      Sums *to = all + part * warps + (threadIdx.x >> 5);
+      store_at(&to->m, lane, mine.m);
+      store_at(&to->s, lane, mine.s);
+      if (ENT) store_at(&to->t, lane, mine.t);
+    }
+    cluster_sync();
+  }
+  Sums v = lane < n ? all[lane] : Sums{};
+  if (n > 32 && lane + 32 < n) join<ENT>(v, all[lane + 32]);
+  return warp_join<ENT>(v);
+}
+
 // ---------------------------------------------------------------------------
 // The likeliest tokens.  An element's key orders the row: the larger value
 // first, of equal ones the lower index, NaNs last; 0 is no element.
@@ -195,65 +322,165 @@ __device__ __forceinline__ float value_of(Key k) {
 }
 __device__ __forceinline__ Key key_of(float v, unsigned index) { return Key(ordered(v)) << 32 | uint32_t(~index); }
 
-constexpr int MAX_TOP = 32, GROUPS = 64, ROOM = 2048;
-struct TopRoom {
+constexpr int MAX_TOP = TC_MAX_TOP, GROUPS = 32;
+static_assert(MAX_TOP <= GROUPS, "a bound needs a group for each of the top tokens");
+template <int ROOM, int THREADS> struct TopRoom {
+  static constexpr int room = ROOM;
   Key group[GROUPS], kept[ROOM], best[MAX_TOP], least;
-  unsigned holder[512], holders, count;
+  float value[GROUPS], bound;
+  unsigned holders, count;
+  unsigned short holder[THREADS];
 };
 
-// The `k` largest keys of a row, in order, into room.best.  `mine` is the
-// key of the thread's largest element and `m` a value that none of its
-// elements passes.  The k-th largest of the largest keys of 64 groups of
-// threads is a bound that k elements at least reach; in rows without
-// structure few more do, and only threads with a maximum that large hold
-// them.  Those threads' elements are read again, the ones that reach the
-// bound are kept and ranked by counting.
-template <class T>
-__device__ __forceinline__ void top_of_row(const typename T::S *row, const Cut<T> &c, Key mine, float m, unsigned k,
-                                           TopRoom &room) {
+// hit(i, rank): the rank of each of `n` values among them, the largest first
+// and of equal ones the first; a warp compares a value with 32 at a time.
+template <class V, class Hit>
+__device__ __forceinline__ void rank_all(const V *value, unsigned n, unsigned warp, unsigned warps, Hit &&hit) {
+  const unsigned lane = threadIdx.x & 31;
+  for (unsigned i = warp; i < n; i += warps) {
+    const V own = value[i];
+    unsigned rank = 0;
+    for (unsigned j = lane; j < (n + 31) / 32 * 32; j += 32)
+      rank += __popc(__ballot_sync(0xffffffffu, j < n && (value[j] > own || (value[j] == own && j < i))));
+    if (lane == 0) hit(i, rank);
+  }
+}
+// The same of distinct keys, for ranks below k alone.
+template <class Hit>
+__device__ __forceinline__ void rank_first(const Key *key, unsigned n, unsigned k, unsigned t, unsigned threads, Hit &&hit) {
+  if (n <= 64) {
+    rank_all(key, n, t >> 5, threads >> 5, [&](unsigned i, unsigned rank) {
+      if (rank < k) hit(i, rank);
+    });
+    return;
+  }
+  for (unsigned i = t; i < n; i += threads) {  // most are soon known to be none of the first k
+    const Key own = key[i];
+    unsigned rank = 0;
+    for (unsigned j = 0; j < n && rank < k; ++j) rank += key[j] > own;
+    if (rank < k) hit(i, rank);
+  }
+}
+
+// Where a thread's largest element was met: in the `runs` runs (each
+// `threads` after the other) of which the first begins at element `at`, or,
+// with runs = 0, at that element (~0: the thread has none).
+struct Met {
+  unsigned at, runs;
+};
+
+// The `k` largest keys of a row (or of a block's part of it: fewer may be
+// there, 0 stands for none), in order, into room.best.  `m` is the thread's
+// largest element, met at `met`; `clean` says that no NaN is among its
+// elements.  The threads are a block's, or (WARP) a warp's.
+//
+// Each of 32 groups of threads has an element as large as its largest, so
+// the k-th largest of those bounds the k-th element of the row from below; in
+// rows without structure few elements more reach it, and only threads whose
+// largest does (the holders) hold any.  Among equal values the index decides:
+// the holders look up where their largest lies, and the k-th largest key of
+// the groups, or of the holders where ties make those many, is the bound
+// that elements are kept by.  The holders' elements are read again (from L2)
+// and the kept ones ranked by counting.
+template <class T, bool WARP, class Room>
+__device__ __forceinline__ void top_of_row(const typename T::S *row, const Cut<T> &c, Met met, float m, bool clean,
+                                           unsigned k, Room &room) {
   using S = typename T::S;
   constexpr unsigned V = Cut<T>::V;
+  const unsigned t = WARP ? threadIdx.x & 31 : threadIdx.x, threads = WARP ? 32 : blockDim.x, lanes = threads / GROUPS;
+  const unsigned warp = t >> 5, warps = threads >> 5;
   const auto load = from_row<T>(row, c);
-  const unsigned t = threadIdx.x, threads = blockDim.x, lanes = threads / GROUPS;
-  Key g = mine;
+  auto sync = [] {
+    if (WARP) __syncwarp();
+    else __syncthreads();
+  };
+  float top = m;
+  for (unsigned o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (t % lanes == 0) room.value[t / lanes] = top;
+  if (t == 0) room.holders = room.count = 0;
+  sync();
+  rank_all(room.value, GROUPS, warp, warps, [&](unsigned i, unsigned rank) {
+    if (rank == k - 1) room.bound = room.value[i];
+  });
+  sync();
+  Key g = 0;
+  if (m >= room.bound && met.at != ~0u) {
+    room.holder[atomicAdd(&room.holders, 1u)] = (unsigned short)t;
+    if (m != -INFINITY) {
+      unsigned at = met.at;
+      for (unsigned u = met.runs; u-- > 0;) {
+        const unsigned i = (met.at - c.body) / V + u * threads;
+        const Bits<T> r = load(i);
+#pragma unroll
+        for (int j = int(V) - 1; j >= 0; --j)
+          if (r.at(j) == m) at = c.body + i * V + unsigned(j);
+      }
+      g = key_of(m, at);
+    } else if (clean) {  // all are -inf, the first among them
+      g = key_of(m, met.at);
+    }
+  }
+  const Key own = g;
   for (unsigned o = 1; o < lanes; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
   if (t % lanes == 0) room.group[t / lanes] = g;
-  if (t == 0) room.holders = room.count = 0;
-  __syncthreads();
-  if (t < GROUPS) {
-    unsigned rank = 0;
-    const Key own = room.group[t];
-    for (unsigned i = 0; i < GROUPS; ++i) rank += room.group[i] > own || (room.group[i] == own && i < t);
-    if (rank == k - 1) room.least = own;
+  sync();
+  rank_all(room.group, GROUPS, warp, warps, [&](unsigned i, unsigned rank) {
+    if (rank == k - 1) room.least = room.group[i];
+  });
+  sync();
+  const unsigned holders = room.holders;
+  if (!WARP && holders > 2 * GROUPS) {
+    // many equal values: the k-th largest of the holders' own keys
+    if (own >= room.least && own) {
+      const unsigned slot = atomicAdd(&room.count, 1u);
+      if (slot < unsigned(Room::room)) room.kept[slot] = own;
+    }
+    __syncthreads();
+    const unsigned n = room.count;
+    __syncthreads();
+    if (n >= k && n <= unsigned(Room::room))
+      rank_first(room.kept, n, k, t, threads, [&](unsigned i, unsigned rank) {
+        if (rank == k - 1) room.least = room.kept[i];
+      });
+    if (t == 0) room.count = 0;
+    __syncthreads();
   }
-  __syncthreads();
   const Key least = room.least;
-  if ((Key(ordered(m)) << 32 | 0xffffffffu) >= least) room.holder[atomicAdd(&room.holders, 1u)] = t;
+  const float bound = value_of(least);  // a NaN where any element may be kept
+  const unsigned limit = ~uint32_t(least);  // of equal values, the last index to be kept
   auto keep = [&](unsigned at, float v) {
+    if (v < bound) return;
     const Key key = key_of(v, at);
     if (key < least) return;
     const unsigned slot = atomicAdd(&room.count, 1u);
-    if (slot < ROOM) room.kept[slot] = key;
+    if (slot < unsigned(Room::room)) room.kept[slot] = key;
   };
-  if (t < c.head) keep(t, T::load(row[t]));
-  if (t < c.tail) keep(c.after + t, T::load(row[c.after + t]));
-  __syncthreads();
-  for (unsigned h = t >> 5; h < room.holders; h += threads >> 5)
-    for (size_t i = room.holder[h] + size_t(t & 31) * threads; i < c.runs; i += size_t(threads) * 32) {
-      const Bits<T> r = load(unsigned(i));
+  auto keep_run = [&](unsigned i, const Bits<T> &r) {
+    const Bits<T> one[1] = {r};
+    const float top = largest(one);
+    if (top < bound || (top == bound && c.body + i * V > limit)) return;
 #pragma unroll
-      for (unsigned j = 0; j < V; ++j) keep(c.body + unsigned(i) * V + j, r.at(j));
-    }
-  __syncthreads();
+    for (unsigned j = 0; j < V; ++j) keep(c.body + i * V + j, r.at(j));
+  };
+  if (holders > threads / 8) {
+    walk<T>(row, c, t, threads, load, [&](unsigned at, S e) { keep(at, T::load(e)); }, [&](unsigned i, const auto &r) {
+      constexpr int U = sizeof(r) / sizeof(r[0]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) keep_run(i + u * threads, r[u]);
+    });
+  } else {
+    if (t < c.head) keep(t, T::load(row[t]));
+    if (t < c.tail) keep(c.after + t, T::load(row[c.after + t]));
+    for (unsigned h = warp; h < holders; h += warps)
+      for (size_t i = room.holder[h] + size_t(t & 31) * threads; i < c.runs; i += size_t(threads) * 32)
+        keep_run(unsigned(i), load(unsigned(i)));
+  }
+  sync();
   const unsigned count = room.count;
-  if (count <= ROOM) {
-    for (unsigned i = t; i < count; i += threads) {
-      const Key own = room.kept[i];
-      unsigned rank = 0;
-      for (unsigned j = 0; j < count; ++j) rank += room.kept[j] > own;
-      if (rank < k) room.best[rank] = own;
-    }
-    __syncthreads();
+  if (count <= unsigned(Room::room)) {
+    for (unsigned i = count + t; i < k; i += threads) room.best[i] = 0;
+    rank_first(room.kept, count, k, t, threads, [&](unsigned i, unsigned rank) { room.best[rank] = room.kept[i]; });
+    sync();
     return;
   }
   // More than there is room for (a row with many NaNs, or whose large values
@@ -275,14 +502,14 @@ __device__ __forceinline__ void top_of_row(const typename T::S *row, const Cut<T
     walk<T>(row, c, t, threads, load, [&](unsigned at, S e) { each(at, T::load(e)); }, many);
 #pragma unroll
     for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if ((t & 31) == 0) room.group[t >> 5] = best;
-    __syncthreads();
-    for (unsigned w = 0; w < threads >> 5; ++w) best = max(best, room.group[w]);
-    __syncthreads();
+    if ((t & 31) == 0) room.group[warp] = best;
+    sync();
+    for (unsigned w = 0; w < warps; ++w) best = max(best, room.group[w]);
+    sync();
     if (t == 0) room.best[n] = best;
     last = best;
   }
-  __syncthreads();
+  sync();
 }
 
 // ---------------------------------------------------------------------------
@@ -291,6 +518,10 @@ __device__ __forceinline__ void top_of_row(const typename T::S *row, const Cut<T
 struct Slope {
   float base, log_sum, entropy, u, v;  // u, v: the gradients of the logprob and of the entropy
   unsigned token;
+  // With p = 2^(a - off), a = x log2(e) - mark, off what rounding the mark
+  // shifted it by: the gradient is 2^a (k1 a + k2).
+  bool wild;
+  float mark, k1, k2;
 };
 template <bool ENT> __device__ __forceinline__ float slope_at(const Slope &g, float x, unsigned at) {
   const float a = (x - g.base) - g.log_sum, p = exp_of(a);
@@ -299,7 +530,14 @@ template <bool ENT> __device__ __forceinline__ float slope_at(const Slope &g, fl
   if (ENT) d -= g.v * p * (fmaxf(a, -1e30f) + g.entropy);
   return d;
 }
-template <bool ENT> __device__ __forceinline__ F2 slope_of_pair(const Slope &g, F2 x) {
+template <bool ENT, bool WILD> __device__ __forceinline__ F2 slope_of_pair(const Slope &g, F2 x) {
+  if constexpr (!WILD) {
+    const F2 a = fma2(x, pair(LOG2E, LOG2E), pair(-g.mark, -g.mark));
+    const float2 y = split(a);
+    const F2 p = pair(exp2_of(y.x), exp2_of(y.y));
+    if (!ENT) return mul2(p, pair(g.k2, g.k2));
+    return mul2(p, fma2(pair(fmaxf(y.x, -1e30f), fmaxf(y.y, -1e30f)), pair(g.k1, g.k1), pair(g.k2, g.k2)));
+  }
   const F2 a = add2(add2(x, pair(-g.base, -g.base)), pair(-g.log_sum, -g.log_sum));
   const float2 y = split(mul2(a, pair(LOG2E, LOG2E)));
   const F2 p = pair(exp2_of(y.x), exp2_of(y.y));
@@ -309,62 +547,82 @@ template <bool ENT> __device__ __forceinline__ F2 slope_of_pair(const Slope &g, 
   const F2 c = add2(pair(fmaxf(z.x, -1e30f), fmaxf(z.y, -1e30f)), pair(g.entropy, g.entropy));
   return mul2(p, fma2(c, pair(-g.v, -g.v), pair(-g.u, -g.u)));
 }
-// load(i) gives the row's run i; elements before and after the runs, and the
-// token's, are read from the row.
-template <class T, bool ENT, class Load>
-__device__ __forceinline__ void write_slope(const typename T::S *row, typename T::S *to, const Cut<T> &c, const Slope &g,
-                                            unsigned t, unsigned threads, Load &&load) {
+// The gradient at the run that begins at element `at`.
+template <class T, bool ENT, bool WILD> __device__ __forceinline__ uint4 slope_run(const Slope &g, const Bits<T> &r, unsigned at) {
   using S = typename T::S;
   constexpr unsigned V = Cut<T>::V;
-  const bool whole = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(to)) & 15) == 0;
-  auto put = [&](unsigned at, uint4 w) {
-    if (whole) {
-      *reinterpret_cast<uint4 *>(to + at) = w;
-    } else {
-      union {
-        uint4 w;
-        S e[V];
-      } u;
-      u.w = w;
+  F2 d[V / 2];
 #pragma unroll
-      for (unsigned j = 0; j < V; ++j) to[at + j] = u.e[j];
-    }
-  };
-  if (g.u == 0.0f && (!ENT || g.v == 0.0f)) {
-    // nothing flows back through this row, whatever its logits
-    if (t < c.head) to[t] = S(0);
-    for (unsigned i = t; i < c.runs; i += threads) put(c.body + i * V, make_uint4(0, 0, 0, 0));
-    if (t < c.tail) to[c.after + t] = S(0);
+  for (unsigned j = 0; j < V / 2; ++j) d[j] = slope_of_pair<ENT, WILD>(g, r.pair_at(j));
+  union {
+    uint4 w;
+    S e[V];
+  } out;
+  if constexpr (T::code == TC_F32) {
+    const float2 lo = split(d[0]), hi = split(d[1]);
+    out.w = make_uint4(__float_as_uint(lo.x), __float_as_uint(lo.y), __float_as_uint(hi.x), __float_as_uint(hi.y));
+  } else {
+    out.w = make_uint4(narrow2<T>(d[0]), narrow2<T>(d[1]), narrow2<T>(d[2]), narrow2<T>(d[3]));
+  }
+  if (g.token - at < V) {
+    const S special = T::store(slope_at<ENT>(g, r.at(g.token - at), g.token));
+#pragma unroll
+    for (unsigned j = 0; j < V; ++j)
+      if (at + j == g.token) out.e[j] = special;
+  }
+  return out.w;
+}
+// A run of the gradient's row, whole where it lies on the grid as the logits do.
+template <class T> __device__ __forceinline__ void put_run(typename T::S *to, uint4 w, bool whole) {
+  using S = typename T::S;
+  if (whole) {
+    __stcs(reinterpret_cast<uint4 *>(to), w);
+  } else {
+    union {
+      uint4 w;
+      S e[Cut<T>::V];
+    } u;
+    u.w = w;
+#pragma unroll
+    for (unsigned j = 0; j < Cut<T>::V; ++j) to[j] = u.e[j];
+  }
+}
+__device__ __forceinline__ bool same_grid(const void *a, const void *b) {
+  return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0;
+}
+template <bool ENT> __device__ __forceinline__ bool no_slope(const Slope &g) { return g.u == 0.0f && (!ENT || g.v == 0.0f); }
+// Nothing flows back through this row, whatever its logits.
+template <class T>
+__device__ __forceinline__ void write_zeros(typename T::S *to, const Cut<T> &c, unsigned t, unsigned threads, bool whole) {
+  using S = typename T::S;
+  if (t < c.head) to[t] = S(0);
+  for (unsigned i = t; i < c.runs; i += threads) put_run<T>(to + c.body + size_t(i) * Cut<T>::V, make_uint4(0, 0, 0, 0), whole);
+  if (t < c.tail) to[c.after + t] = S(0);
+}
+template <class T, bool ENT>
+__device__ __forceinline__ void write_slope(const typename T::S *row, typename T::S *to, const Cut<T> &c, const Slope &g,
+                                            unsigned t, unsigned threads) {
+  using S = typename T::S;
+  constexpr unsigned V = Cut<T>::V;
+  const bool whole = same_grid(row, to);
+  if (no_slope<ENT>(g)) {
+    write_zeros<T>(to, c, t, threads, whole);
     return;
   }
-  auto many = [&](unsigned i, const auto &r) {
-    constexpr int U = sizeof(r) / sizeof(r[0]);
+  auto write = [&](auto wild) {
+    walk<T>(
+        row, c, t, threads, from_row<T>(row, c), [&](unsigned at, S e) { to[at] = T::store(slope_at<ENT>(g, T::load(e), at)); },
+        [&](unsigned i, const auto &r) {
+          constexpr int U = sizeof(r) / sizeof(r[0]);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const unsigned at = c.body + (i + u * threads) * V;
-      F2 d[V / 2];
-#pragma unroll
-      for (unsigned j = 0; j < V / 2; ++j) d[j] = slope_of_pair<ENT>(g, r[u].pair_at(j));
-      union {
-        uint4 w;
-        S e[V];
-      } out;
-      if constexpr (T::code == TC_F32) {
-        const float2 lo = split(d[0]), hi = split(d[1]);
-        out.w = make_uint4(__float_as_uint(lo.x), __float_as_uint(lo.y), __float_as_uint(hi.x), __float_as_uint(hi.y));
-      } else {
-        out.w = make_uint4(narrow2<T>(d[0]), narrow2<T>(d[1]), narrow2<T>(d[2]), narrow2<T>(d[3]));
-      }
-      if (g.token - at < V) {
-        const S special = T::store(slope_at<ENT>(g, r[u].at(g.token - at), g.token));
-#pragma unroll
-        for (unsigned j = 0; j < V; ++j)
-          if (at + j == g.token) out.e[j] = special;
-      }
-      put(at, out.w);
-    }
+          for (int u = 0; u < U; ++u) {
+            const unsigned at = c.body + (i + u * threads) * V;
+            put_run<T>(to + at, slope_run<T, ENT, decltype(wild)::value>(g, r[u], at), whole);
+          }
+        });
   };
-  walk<T>(row, c, t, threads, load, [&](unsigned at, S e) { to[at] = T::store(slope_at<ENT>(g, T::load(e), at)); }, many);
+  if (g.wild) write(std::true_type{});
+  else write(std::false_type{});
 }
 
 struct TokenArgs {
@@ -393,88 +651,317 @@ __device__ __forceinline__ Slope slope_of(const TokenArgs &a, size_t r, float2 s
   g.token = a.tokens ? a.tokens[r] : ~0u;
   g.u = a.grad_logprobs && g.token < a.vocab && !empty ? a.grad_logprobs[r] : 0.0f;
   g.v = a.grad_entropy && !empty ? a.grad_entropy[r] : 0.0f;
+  g.wild = !tame(g.base);
+  g.mark = fmaf(g.base, LOG2E, g.log_sum * LOG2E);
+  const float off = fmaf(g.base, LOG2E, -g.mark) + g.log_sum * LOG2E, f = exp2_of(-off);
+  g.k1 = -g.v * LN2 * f;
+  g.k2 = -(g.u + g.v * (g.entropy - off * LN2)) * f;
   return g;
+}
+
+// What a row's sums say.
+struct Told {
+  float2 st;
+  float entropy;
+};
+template <bool ENT> __device__ __forceinline__ Told told_by(const Sums &all) {
+  const bool empty = all.m == -INFINITY && all.s == 0.0f;
+  Told o;
+  o.st = make_float2(all.m, empty ? 0.0f : logf(all.s));
+  o.entropy = !ENT || empty ? 0.0f : o.st.y - all.t / all.s;
+  return o;
+}
+// `at_token` is the token's logit, read before any gradient is written.
+template <bool ENT>
+__device__ __forceinline__ void write_told(const TokenArgs &a, size_t r, const Told &o, unsigned token, float at_token) {
+  if (a.logprobs) a.logprobs[r] = token == ~0u ? 0.0f : (at_token - base_of(o.st.x)) - o.st.y;
+  if (a.statistics) a.statistics[r] = o.st;
+  if (ENT && a.entropy) a.entropy[r] = o.entropy;
+}
+__device__ __forceinline__ void write_top(const TokenArgs &a, size_t r, const Told &o, unsigned i, Key k) {
+  a.top_tokens[r * a.top + i] = ~uint32_t(k);
+  a.top_logprobs[r * a.top + i] = (value_of(k) - base_of(o.st.x)) - o.st.y;
+}
+template <class T> __device__ __forceinline__ float logit_of(const typename T::S *row, unsigned token, unsigned vocab) {
+  return token < vocab ? T::load(row[token]) : __int_as_float(0x7fc00000);
 }
 
 enum Extra { NOTHING = 0, TOP = 1, GRADIENT = 2 };
 
-// A block a row: the statistics in one pass, and then what is asked for.
-template <class T, bool ENT, int EXTRA> __global__ void __launch_bounds__(512) token_rows(TokenArgs a) {
+// Small vocabularies: a warp holds a row, U runs a lane.  The row is read
+// once, whatever is asked for but the top tokens' second look.
+template <class T, bool ENT, int EXTRA, int U> __global__ void __launch_bounds__(256) token_small(const TokenArgs a) {
   using S = typename T::S;
   constexpr unsigned V = Cut<T>::V;
-  __shared__ Sums room[16];
-  const unsigned t = threadIdx.x, threads = blockDim.x;
-  for (size_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+  constexpr uint32_t LOW = T::code == TC_F32 ? 0xff800000u : T::code == TC_BF16 ? 0xff80ff80u : 0xfc00fc00u;  // -inf
+  const unsigned lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  __shared__ std::conditional_t<EXTRA == TOP, TopRoom<256, 32>, int> rooms[EXTRA == TOP ? 8 : 1];
+  for (size_t r = size_t(blockIdx.x) * warps + (threadIdx.x >> 5); r < a.rows; r += size_t(gridDim.x) * warps) {
     const S *row = static_cast<const S *>(a.logits) + r * a.stride;
     const Cut<T> c(row, a.vocab);
     const unsigned token = a.tokens ? a.tokens[r] : ~0u;
-    const float at_token = token < a.vocab ? T::load(row[token]) : __int_as_float(0x7fc00000);
+    const float at_token = logit_of<T>(row, token, a.vocab);
+    Bits<T> bits[U];
+    const auto load = from_row<T>(row, c);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      bits[u].w = make_uint4(LOW, LOW, LOW, LOW);
+      if (lane + 32 * u < c.runs) bits[u] = load(lane + 32 * u);
+    }
+    // the single elements: those before the runs to the first lanes, those
+    // after them from lane 8 on
+    const unsigned single = lane < c.head ? lane : lane >= 8 && lane - 8 < c.tail ? c.after + lane - 8 : ~0u;
+    const float extra = single != ~0u ? T::load(row[single]) : -INFINITY;
+    const float in_runs = largest(bits), m = fmaxf(in_runs, extra);
+    float all_m = m;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) all_m = fmaxf(all_m, __shfl_xor_sync(0xffffffffu, all_m, o));
     Running<T, ENT> run;
-    // where the thread's largest element lies; its first, while all are -inf
-    unsigned at = t < c.head ? t : t < c.runs ? c.body + t * V : t < c.tail ? c.after + t : ~0u;
-    auto one = [&](unsigned i, S e) {
-      const float v = T::load(e);
-      if (v > run.m) {
-        run.lift(v);
-        if (EXTRA == TOP) at = i;
+    run.begin(all_m);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (32 * u < int(c.runs)) {
+        const Bits<T> one[1] = {bits[u]};
+        run.add(one);
       }
-      run.add(pair(v, -INFINITY));
-    };
-    auto many = [&](unsigned i, const auto &bits) {
-      constexpr int U = sizeof(bits) / sizeof(bits[0]);
-      const float m = largest(bits);
-      if (m > run.m) {
-        run.lift(m);
-        if (EXTRA == TOP) {
+    run.add_one(extra);
+    Sums sums = run.sums();
+    const bool clean = !isnan(sums.s);
 #pragma unroll
-          for (int u = U - 1; u >= 0; --u)
+    for (int o = 16; o; o >>= 1) {
+      sums.s += __shfl_xor_sync(0xffffffffu, sums.s, o);
+      if (ENT) sums.t += __shfl_xor_sync(0xffffffffu, sums.t, o);
+    }
+    const Told o = told_by<ENT>(sums);
+    if (lane == 0) write_told<ENT>(a, r, o, token, at_token);
+    if constexpr (EXTRA == TOP) {
+      auto &room = rooms[threadIdx.x >> 5];
+      const unsigned mine = lane < c.runs ? (c.runs - lane + 31) / 32 : 0;
+      Met met{c.body + lane * V, mine};
+      if (single != ~0u && (mine == 0 || (lane < c.head ? extra >= in_runs : extra > in_runs))) met = Met{single, 0};
+      else if (mine == 0) met = Met{~0u, 0};
+      top_of_row<T, true>(row, c, met, m, clean, a.top, room);
+      if (lane < a.top) write_top(a, r, o, lane, room.best[lane]);
+      __syncwarp();
+    }
+    if constexpr (EXTRA == GRADIENT) {
+      const Slope g = slope_of(a, r, o.st, o.entropy);
+      S *to = static_cast<S *>(a.grad_logits) + r * a.grad_stride;
+      const bool whole = same_grid(row, to), none = no_slope<ENT>(g);
+      auto write = [&](auto wild) {
 #pragma unroll
-            for (int j = int(V) - 1; j >= 0; --j)
-              if (bits[u].at(j) == m) at = c.body + (i + u * threads) * V + unsigned(j);
+        for (int u = 0; u < U; ++u) {
+          const unsigned i = lane + 32 * u, at = c.body + i * V;
+          if (i < c.runs)
+            put_run<T>(to + at, none ? make_uint4(0, 0, 0, 0) : slope_run<T, ENT, decltype(wild)::value>(g, bits[u], at), whole);
         }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (unsigned j = 0; j < V / 2; ++j) run.add(bits[u].pair_at(j));
-    };
-    walk<T>(row, c, t, threads, from_row<T>(row, c), one, many);
-    const Sums sums = run.sums();
-    const Sums all = block_join<ENT>(sums, room);
-    const bool empty = all.m == -INFINITY && all.s == 0.0f;
-    const float2 st = make_float2(all.m, empty ? 0.0f : logf(all.s));
-    const float entropy = !ENT || empty ? 0.0f : st.y - all.t / all.s;
-    if (t == 0) {
-      if (a.logprobs) a.logprobs[r] = token == ~0u ? 0.0f : (at_token - base_of(st.x)) - st.y;
-      if (a.statistics) a.statistics[r] = st;
-      if (ENT && a.entropy) a.entropy[r] = entropy;
+      };
+      if (g.wild) write(std::true_type{});
+      else write(std::false_type{});
+      if (single != ~0u) to[single] = none ? S(0) : T::store(slope_at<ENT>(g, extra, single));
     }
-    if (EXTRA == TOP) {
-      __shared__ TopRoom top;
-      // a NaN among the thread's elements: `at` may not name one of value m
-      const Key mine = at == ~0u || isnan(sums.s) ? 0 : key_of(sums.m, at);
-      top_of_row<T>(row, c, mine, sums.m, a.top, top);
-      if (t < a.top) {
-        const Key k = top.best[t];
-        a.top_tokens[r * a.top + t] = ~uint32_t(k);
-        a.top_logprobs[r * a.top + t] = (value_of(k) - base_of(st.x)) - st.y;
-      }
-    }
-    if (EXTRA == GRADIENT)
-      write_slope<T, ENT>(row, static_cast<S *>(a.grad_logits) + r * a.grad_stride, c, slope_of(a, r, st, entropy), t, threads, from_row<T>(row, c));
-    __syncthreads();
   }
 }
 
-// The gradient alone, from the statistics that the forward call left.
-template <class T, bool ENT> __global__ void __launch_bounds__(512) token_slope(TokenArgs a) {
+// A thread's runs of the rows that its block takes, copied ahead of their use
+// into slots of its own (so only it waits for them): `groups` groups of four,
+// as many as a row has.
+template <class T> struct Ahead {
   using S = typename T::S;
-  for (size_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+  const TokenArgs &a;
+  uint4 *const slots;
+  const unsigned t, threads, groups;
+  size_t row;            // of the next group
+  unsigned group, runs;  // of the row; the row's
+  const uint4 *from;
+  __device__ __forceinline__ Ahead(const TokenArgs &a, void *slots, unsigned groups)
+      : a(a), slots(static_cast<uint4 *>(slots) + threadIdx.x), t(threadIdx.x), threads(blockDim.x), groups(groups),
+        row(blockIdx.x), group(0) {
+    place();
+  }
+  __device__ __forceinline__ void place() {
+    if (row >= a.rows) return;
+    const S *at = static_cast<const S *>(a.logits) + row * a.stride;
+    const Cut<T> c(at, a.vocab);
+    from = reinterpret_cast<const uint4 *>(at + c.body) + t;
+    runs = c.runs;
+  }
+  __device__ __forceinline__ uint4 *slot(unsigned g, int u) const { return slots + (g * 4 + u) * threads; }
+  // Begin the next group's copies; the group of the row before it is no
+  // longer needed.
+  __device__ __forceinline__ void fetch() {
+    if (row < a.rows) {
+      const unsigned i = group * 4 * threads;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (t + i + u * threads < runs) copy_async(uint32_t(__cvta_generic_to_shared(slot(group, u))), from + i + u * threads);
+      if (++group == groups) {
+        group = 0;
+        row += gridDim.x;
+        place();
+      }
+    }
+    copy_commit();
+  }
+  // A thread's part of a group that has arrived: f(first run, bits[1 or 4])
+  // for the runs that it has.
+  template <class F> __device__ __forceinline__ void each(unsigned g, const Cut<T> &c, F &&f) const {
+    const unsigned i = t + g * 4 * threads;
+    if (i + 3 * threads < c.runs) {
+      Bits<T> r[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) r[u].w = *slot(g, u);
+      f(i, r);
+    } else {
+      for (int u = 0; u < 4; ++u)
+        if (i + u * threads < c.runs) {
+          Bits<T> r[1];
+          r[0].w = *slot(g, u);
+          f(i + u * threads, r);
+        }
+    }
+  }
+};
+
+// Larger ones: a block a row, or a cluster's blocks, each a part of it.
+template <class T, bool ENT, int EXTRA> __global__ void __launch_bounds__(256, 6) token_rows(const TokenArgs a) {
+  using S = typename T::S;
+  constexpr unsigned V = Cut<T>::V;
+  __shared__ Slots joint;
+  const unsigned t = threadIdx.x, threads = blockDim.x, part = cluster_part(), parts = cluster_parts();
+  const size_t first = blockIdx.x / parts, step = gridDim.x / parts;
+  unsigned turn = 0;
+  for (size_t r = first; r < a.rows; r += step, turn ^= 1) {
+    const S *row = static_cast<const S *>(a.logits) + r * a.stride;
+    const Cut<T> c(row, a.vocab, part, parts);
+    const unsigned token = a.tokens ? a.tokens[r] : ~0u;
+    const float at_token = part == 0 && t == 0 ? logit_of<T>(row, token, a.vocab) : 0.0f;
+    Running<T, ENT> run;
+    // the thread's first element, while all are -inf; none: ~0
+    Met met{t < c.head ? t : t < c.runs ? c.body + t * V : t < c.tail ? c.after + t : ~0u, 0};
+    walk<T>(
+        row, c, t, threads, from_row<T>(row, c),
+        [&](unsigned i, S e) {
+          if (run.take_one(T::load(e))) met = Met{i, 0};
+        },
+        [&](unsigned i, const auto &bits) {
+          if (run.take(bits)) met = Met{c.body + i * V, unsigned(sizeof(bits) / sizeof(bits[0]))};
+        });
+    const Sums sums = run.sums();
+    const Sums all = row_join<ENT>(sums, joint, part, parts, turn);
+    const Told o = told_by<ENT>(all);
+    if (part == 0 && t == 0) write_told<ENT>(a, r, o, token, at_token);
+    if constexpr (EXTRA == TOP) {
+      __shared__ TopRoom<1024, 256> top;
+      __shared__ Key parts_best[8 * MAX_TOP];
+      top_of_row<T, false>(row, c, met, sums.m, !isnan(sums.s), a.top, top);
+      if (parts == 1) {
+        if (t < a.top) write_top(a, r, o, t, top.best[t]);
+      } else {
+        // each block's top tokens to the first, which has the row's among them
+        if (t < a.top) store_at(&parts_best[part * a.top + t], 0, top.best[t]);
+        cluster_sync();
+        if (part == 0) {
+          const unsigned n = parts * a.top;
+          for (unsigned i = t; i < n; i += threads) {
+            const Key own = parts_best[i];
+            unsigned rank = 0;
+            for (unsigned j = 0; j < n; ++j) rank += parts_best[j] > own;
+            if (rank < a.top && own) write_top(a, r, o, rank, own);
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// The loss of rows that a block's shared memory holds: a row stays in its
+// slots until its gradient is written from there, and the next one follows it
+// group by group.
+template <class T, bool ENT> __global__ void __launch_bounds__(256, 3) token_loss_held(const TokenArgs a, unsigned groups) {
+  using S = typename T::S;
+  constexpr unsigned V = Cut<T>::V;
+  extern __shared__ __align__(16) unsigned char slots[];
+  __shared__ Slots joint;
+  const unsigned t = threadIdx.x, threads = blockDim.x;
+  Ahead<T> ring(a, slots, groups);
+  for (unsigned g = 0; g < groups; ++g) ring.fetch();
+  unsigned turn = 0;
+  for (size_t r = blockIdx.x; r < a.rows; r += gridDim.x, turn ^= 1) {
+    const S *row = static_cast<const S *>(a.logits) + r * a.stride;
+    const Cut<T> c(row, a.vocab);
+    const unsigned token = a.tokens ? a.tokens[r] : ~0u;
+    const float at_token = t == 0 ? logit_of<T>(row, token, a.vocab) : 0.0f;
+    Running<T, ENT> run;
+    copy_wait<0>();
+    if (t < c.head) run.take_one(T::load(row[t]));
+    for (unsigned g = 0; g < groups; ++g) ring.each(g, c, [&](unsigned, const auto &bits) { run.take(bits); });
+    if (t < c.tail) run.take_one(T::load(row[c.after + t]));
+    const Told o = told_by<ENT>(row_join<ENT>(run.sums(), joint, 0, 1, turn));
+    if (t == 0) write_told<ENT>(a, r, o, token, at_token);
+    const Slope s = slope_of(a, r, o.st, o.entropy);
+    S *to = static_cast<S *>(a.grad_logits) + r * a.grad_stride;
+    const bool whole = same_grid(row, to), none = no_slope<ENT>(s);
+    if (none) {
+      write_zeros<T>(to, c, t, threads, whole);
+    } else {
+      if (t < c.head) to[t] = T::store(slope_at<ENT>(s, T::load(row[t]), t));
+      if (t < c.tail) to[c.after + t] = T::store(slope_at<ENT>(s, T::load(row[c.after + t]), c.after + t));
+    }
+    auto write = [&](auto wild) {
+      for (unsigned g = 0; g < groups; ++g) {
+        if (!none)
+          ring.each(g, c, [&](unsigned i, const auto &bits) {
+            constexpr int U = sizeof(bits) / sizeof(bits[0]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const unsigned at = c.body + (i + u * threads) * V;
+              put_run<T>(to + at, slope_run<T, ENT, decltype(wild)::value>(s, bits[u], at), whole);
+            }
+          });
+        ring.fetch();
+      }
+    };
+    if (s.wild) write(std::true_type{});
+    else write(std::false_type{});
+  }
+}
+
+// Larger rows, and few: the blocks of a cluster share a row, and the second
+// pass reads it from L2, which the parts of all resident blocks leave room in.
+template <class T, bool ENT> __global__ void __launch_bounds__(256, 4) token_loss_twice(const TokenArgs a) {
+  using S = typename T::S;
+  __shared__ Slots joint;
+  const unsigned t = threadIdx.x, threads = blockDim.x, part = cluster_part(), parts = cluster_parts();
+  const size_t first = blockIdx.x / parts, step = gridDim.x / parts;
+  unsigned turn = 0;
+  for (size_t r = first; r < a.rows; r += step, turn ^= 1) {
+    const S *row = static_cast<const S *>(a.logits) + r * a.stride;
+    const Cut<T> c(row, a.vocab, part, parts);
+    const unsigned token = a.tokens ? a.tokens[r] : ~0u;
+    const float at_token = part == 0 && t == 0 ? logit_of<T>(row, token, a.vocab) : 0.0f;
+    Running<T, ENT> run;
+    walk<T>(
+        row, c, t, threads, from_row<T>(row, c), [&](unsigned, S e) { run.take_one(T::load(e)); },
+        [&](unsigned, const auto &bits) { run.take(bits); });
+    const Told o = told_by<ENT>(row_join<ENT>(run.sums(), joint, part, parts, turn));
+    if (part == 0 && t == 0) write_told<ENT>(a, r, o, token, at_token);
+    write_slope<T, ENT>(row, static_cast<S *>(a.grad_logits) + r * a.grad_stride, c, slope_of(a, r, o.st, o.entropy), t, threads);
+  }
+}
+
+// The gradient alone, from the statistics that the forward call left, by
+// blocks or (`apart`) by warps of a row each.
+template <class T, bool ENT> __global__ void __launch_bounds__(512) token_slope(const TokenArgs a, bool apart) {
+  using S = typename T::S;
+  const unsigned threads = apart ? 32 : blockDim.x, each = blockDim.x / threads;
+  const unsigned t = apart ? threadIdx.x & 31 : threadIdx.x;
+  for (size_t r = size_t(blockIdx.x) * each + (apart ? threadIdx.x >> 5 : 0); r < a.rows; r += size_t(gridDim.x) * each) {
     const S *row = static_cast<const S *>(a.logits) + r * a.stride;
     const Cut<T> c(row, a.vocab);
     write_slope<T, ENT>(row, static_cast<S *>(a.grad_logits) + r * a.grad_stride, c,
-                        slope_of(a, r, a.kept_statistics[r], ENT ? a.kept_entropy[r] : 0.0f), threadIdx.x, blockDim.x,
-                        from_row<T>(row, c));
+                        slope_of(a, r, a.kept_statistics[r], ENT ? a.kept_entropy[r] : 0.0f), t, threads);
   }
 }
 
@@ -490,9 +977,97 @@ int check(const char *what, size_t rows, size_t vocab, size_t stride, const char
 }
 bool off_grid(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
 
-unsigned threads_for(size_t vocab, size_t run) {
-  const size_t want = vocab / run / 4;
-  return want >= 512 ? 512 : want >= 256 ? 256 : 128;
+// Launch `kernel` in clusters of `parts` blocks.
+template <class... A>
+int launch(const char *what, void (*kernel)(A...), size_t clusters, unsigned parts, unsigned threads, size_t shared,
+           cudaStream_t stream, std::common_type_t<A>... args) {
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = parts;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(unsigned(clusters * parts));
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = shared;
+  config.stream = stream;
+  config.attrs = &cluster;
+  config.numAttrs = parts > 1 ? 1 : 0;
+  return check_cuda(cudaLaunchKernelEx(&config, kernel, args...), what);
+}
+
+// Blocks of `kernel` that the GPU holds at once.
+template <class K> size_t resident(K kernel, unsigned threads, size_t shared) {
+  int n = 0;
+  cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, int(threads), shared);
+  return size_t(std::max(1, n)) * size_t(sm_count());
+}
+
+// In how many parts to cut each of `rows` rows of `runs` runs: as many as
+// leave none of `slots` blocks idle and each thread two runs.  (Cutting
+// further, to even out the blocks' last rows, costs more in joins.)
+unsigned parts_for(size_t rows, size_t runs, unsigned threads, size_t slots) {
+  unsigned parts = 1;
+  while (parts < 8 && rows * parts * 2 <= slots && runs / (parts * 2) >= 2 * threads) parts *= 2;
+  return parts;
+}
+
+// The most runs of a part whose row is read twice: 100 KB a block, of which
+// four blocks on each of 148 SMs hold 60 MB. 4096x131072 bf16 (16384 runs)
+// takes 411 us in four parts, 462 in two, 476 in one; 4096x50257 (6282) 175
+// in one, 181 in two.
+constexpr size_t PART_RUNS = 6400;
+template <class K> int allow_shared(K kernel, size_t most) {
+  return check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most)), "token logprobs");
+}
+
+// A warp a row up to 8 runs a lane; 2 where those do.
+template <class T, bool ENT, int EXTRA> int small(const char *what, const TokenArgs &a, cudaStream_t stream) {
+  const unsigned grid = unsigned(std::min<size_t>((a.rows + 7) / 8, size_t(sm_count()) * 64));
+  if (a.vocab <= 64 * Cut<T>::V) token_small<T, ENT, EXTRA, 2><<<grid, 256, 0, stream>>>(a);
+  else token_small<T, ENT, EXTRA, 8><<<grid, 256, 0, stream>>>(a);
+  return check_launch(what);
+}
+template <class T> bool is_small(const TokenArgs &a) { return a.vocab <= 256 * Cut<T>::V; }
+
+template <class T, bool ENT, bool WITH_TOP> int forward(const TokenArgs &a, cudaStream_t stream) {
+  constexpr int EXTRA = WITH_TOP ? TOP : NOTHING;
+  if (is_small<T>(a)) return small<T, ENT, EXTRA>("token logprobs", a, stream);
+  auto kernel = token_rows<T, ENT, EXTRA>;
+  const size_t runs = a.vocab / Cut<T>::V;
+  const unsigned threads = runs >= 2048 && !WITH_TOP ? 256 : 128;
+  const size_t slots = resident(kernel, threads, 0);
+  const unsigned parts = parts_for(a.rows, runs, threads, slots);
+  return launch("token logprobs", kernel, std::min<size_t>(a.rows, (1u << 30) / parts), parts, threads, 0, stream, a);
+}
+
+template <class T, bool ENT> int loss(const TokenArgs &a, cudaStream_t stream) {
+  if (is_small<T>(a)) return small<T, ENT, GRADIENT>("token loss", a, stream);
+  const size_t runs = a.vocab / Cut<T>::V;
+  const unsigned threads = runs >= 2048 ? 256 : 128;
+  // Sixteen runs a thread leave three blocks on an SM; with fewer rows than
+  // SMs each row is better shared.
+  if (runs <= 16 * size_t(threads) && a.rows > size_t(sm_count())) {
+    auto kernel = token_loss_held<T, ENT>;
+    const size_t groups = (runs + 4 * threads - 1) / (4 * threads), shared = groups * 4 * 16 * threads;
+    static const int allowed = allow_shared(kernel, 16 * 16 * 256);
+    if (allowed) return allowed;
+    const unsigned grid = unsigned(std::min<size_t>(a.rows, resident(kernel, threads, shared)));
+    kernel<<<grid, threads, shared, stream>>>(a, unsigned(groups));
+    return check_launch("token loss");
+  }
+  auto kernel = token_loss_twice<T, ENT>;
+  unsigned parts = parts_for(a.rows, runs, threads, resident(kernel, threads, 0));
+  while (parts < 8 && runs > PART_RUNS * parts) parts *= 2;
+  return launch("token loss", kernel, std::min<size_t>(a.rows, (1u << 30) / parts), parts, threads, 0, stream, a);
+}
+
+template <class T, bool ENT> int backward(const TokenArgs &a, cudaStream_t stream) {
+  const bool apart = is_small<T>(a);
+  const size_t runs = a.vocab / Cut<T>::V;
+  const unsigned threads = apart ? 256 : runs >= 8192 ? 512 : runs >= 2048 ? 256 : 128;
+  const size_t blocks = apart ? (a.rows + 7) / 8 : a.rows;
+  token_slope<T, ENT><<<unsigned(std::min<size_t>(blocks, 1u << 30)), threads, 0, stream>>>(a, apart);
+  return check_launch("token logprobs backward");
 }
 
 }  // namespace
@@ -527,16 +1102,9 @@ int tc_token_logprobs(int dtype, size_t rows, size_t vocab, const void *logits, 
     a.statistics = reinterpret_cast<float2 *>(statistics);
     a.top_tokens = top_tokens;
     a.top_logprobs = top_logprobs;
-    const unsigned grid = unsigned(std::min<size_t>(rows, 1u << 30)), threads = threads_for(vocab, 16 / sizeof(typename T::S));
     cudaStream_t on = as_stream(stream);
-    if (top) {
-      if (entropy) token_rows<T, true, TOP><<<grid, threads, 0, on>>>(a);
-      else token_rows<T, false, TOP><<<grid, threads, 0, on>>>(a);
-    } else {
-      if (entropy) token_rows<T, true, NOTHING><<<grid, threads, 0, on>>>(a);
-      else token_rows<T, false, NOTHING><<<grid, threads, 0, on>>>(a);
-    }
-    return check_launch("token logprobs");
+    return entropy ? (top ? forward<T, true, true>(a, on) : forward<T, true, false>(a, on))
+                   : (top ? forward<T, false, true>(a, on) : forward<T, false, false>(a, on));
   });
 }
 
@@ -565,10 +1133,7 @@ int tc_token_logprobs_backward(int dtype, size_t rows, size_t vocab, const void 
     a.grad_entropy = grad_entropy;
     a.grad_logits = grad_logits;
     a.grad_stride = grad_stride;
-    const unsigned grid = unsigned(std::min<size_t>(rows, 1u << 30)), threads = threads_for(vocab, 16 / sizeof(typename T::S));
-    if (grad_entropy) token_slope<T, true><<<grid, threads, 0, as_stream(stream)>>>(a);
-    else token_slope<T, false><<<grid, threads, 0, as_stream(stream)>>>(a);
-    return check_launch("token logprobs backward");
+    return grad_entropy ? backward<T, true>(a, as_stream(stream)) : backward<T, false>(a, as_stream(stream));
   });
 }
 
@@ -596,10 +1161,7 @@ int tc_token_loss(int dtype, size_t rows, size_t vocab, const void *logits, size
     a.grad_entropy = grad_entropy;
     a.grad_logits = grad_logits;
     a.grad_stride = grad_stride;
-    const unsigned grid = unsigned(std::min<size_t>(rows, 1u << 30)), threads = threads_for(vocab, 16 / sizeof(typename T::S));
-    if (entropy || grad_entropy) token_rows<T, true, GRADIENT><<<grid, threads, 0, as_stream(stream)>>>(a);
-    else token_rows<T, false, GRADIENT><<<grid, threads, 0, as_stream(stream)>>>(a);
-    return check_launch("token loss");
+    return entropy || grad_entropy ? loss<T, true>(a, as_stream(stream)) : loss<T, false>(a, as_stream(stream));
   });
 }
 

@@ -113,17 +113,6 @@ __global__ void __launch_bounds__(1024) norm_rows_wide(const typename T::S *x, s
   }
 }
 
-// Copies 16 bytes from global to shared memory; a thread's copies complete in
-// the order of its commits.
-__device__ __forceinline__ void copy_async(uint32_t to, const void *from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// Until at most LEFT of this thread's last commits are under way.
-template <int LEFT> __device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
-}
-
 // grad_x, and this block's share of grad_w and grad_b.  A block is `groups`
 // groups of `threads` threads; a group takes a turn of R neighbouring rows at
 // a time and its threads own the same columns of every row, so the columns'

@@ -116,6 +116,17 @@ template <class T, int E> __device__ __forceinline__ void load_wide(const typena
   }
 }
 
+// Copies 16 bytes from global to shared memory; a thread's copies complete in
+// the order of its commits.
+__device__ __forceinline__ void copy_async(uint32_t to, const void *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Until at most LEFT of this thread's last commits are under way.
+template <int LEFT> __device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
