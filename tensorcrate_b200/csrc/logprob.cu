@@ -348,7 +348,7 @@ __device__ __forceinline__ void rank_all(const V *value, unsigned n, unsigned wa
 // The same of distinct keys, for ranks below k alone.
 template <class Hit>
 __device__ __forceinline__ void rank_first(const Key *key, unsigned n, unsigned k, unsigned t, unsigned threads, Hit &&hit) {
-  if (n <= 64) {
+  if (n <= 64 && threads > 32) {
     rank_all(key, n, t >> 5, threads >> 5, [&](unsigned i, unsigned rank) {
       if (rank < k) hit(i, rank);
     });
@@ -399,9 +399,19 @@ __device__ __forceinline__ void top_of_row(const typename T::S *row, const Cut<T
   if (t % lanes == 0) room.value[t / lanes] = top;
   if (t == 0) room.holders = room.count = 0;
   sync();
-  rank_all(room.value, GROUPS, warp, warps, [&](unsigned i, unsigned rank) {
-    if (rank == k - 1) room.bound = room.value[i];
-  });
+  if (WARP) {  // a value a lane
+    unsigned rank = 0;
+#pragma unroll 8
+    for (unsigned j = 0; j < 32; ++j) {
+      const float v = __shfl_sync(0xffffffffu, m, j);
+      rank += v > m || (v == m && j < t);
+    }
+    if (rank == k - 1) room.bound = m;
+  } else {
+    rank_all(room.value, GROUPS, warp, warps, [&](unsigned i, unsigned rank) {
+      if (rank == k - 1) room.bound = room.value[i];
+    });
+  }
   sync();
   Key g = 0;
   if (m >= room.bound && met.at != ~0u) {
@@ -424,9 +434,16 @@ __device__ __forceinline__ void top_of_row(const typename T::S *row, const Cut<T
   for (unsigned o = 1; o < lanes; o <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
   if (t % lanes == 0) room.group[t / lanes] = g;
   sync();
-  rank_all(room.group, GROUPS, warp, warps, [&](unsigned i, unsigned rank) {
-    if (rank == k - 1) room.least = room.group[i];
-  });
+  if (WARP) {
+    unsigned rank = 0;
+#pragma unroll 8
+    for (unsigned j = 0; j < 32; ++j) rank += room.group[j] > g || (room.group[j] == g && j < t);
+    if (rank == k - 1) room.least = g;
+  } else {
+    rank_all(room.group, GROUPS, warp, warps, [&](unsigned i, unsigned rank) {
+      if (rank == k - 1) room.least = room.group[i];
+    });
+  }
   sync();
   const unsigned holders = room.holders;
   if (!WARP && holders > 2 * GROUPS) {
@@ -1020,10 +1037,11 @@ template <class K> int allow_shared(K kernel, size_t most) {
   return check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most)), "token logprobs");
 }
 
-// A warp a row up to 8 runs a lane; 2 where those do.
+// A warp a row up to 8 runs a lane; 2 or 4 where those do.
 template <class T, bool ENT, int EXTRA> int small(const char *what, const TokenArgs &a, cudaStream_t stream) {
   const unsigned grid = unsigned(std::min<size_t>((a.rows + 7) / 8, size_t(sm_count()) * 64));
   if (a.vocab <= 64 * Cut<T>::V) token_small<T, ENT, EXTRA, 2><<<grid, 256, 0, stream>>>(a);
+  else if (a.vocab <= 128 * Cut<T>::V) token_small<T, ENT, EXTRA, 4><<<grid, 256, 0, stream>>>(a);
   else token_small<T, ENT, EXTRA, 8><<<grid, 256, 0, stream>>>(a);
   return check_launch(what);
 }
@@ -1034,7 +1052,8 @@ template <class T, bool ENT, bool WITH_TOP> int forward(const TokenArgs &a, cuda
   if (is_small<T>(a)) return small<T, ENT, EXTRA>("token logprobs", a, stream);
   auto kernel = token_rows<T, ENT, EXTRA>;
   const size_t runs = a.vocab / Cut<T>::V;
-  const unsigned threads = runs >= 2048 && !WITH_TOP ? 256 : 128;
+  // the top tokens' steps wait for one another: smaller blocks, more of them
+  const unsigned threads = runs >= 2048 && (!WITH_TOP || a.rows <= size_t(sm_count())) ? 256 : 128;
   const size_t slots = resident(kernel, threads, 0);
   const unsigned parts = parts_for(a.rows, runs, threads, slots);
   return launch("token logprobs", kernel, std::min<size_t>(a.rows, (1u << 30) / parts), parts, threads, 0, stream, a);
