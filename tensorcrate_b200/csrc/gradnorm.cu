@@ -14,17 +14,18 @@
 namespace tc {
 namespace {
 
-// The tensors of one launch travel in the kernel's parameters.  A tensor is
-// cut into chunks of CHUNK bytes, which the launch's blocks take in turn;
-// first[i] is the number of chunks before tensor i.
-constexpr unsigned CHUNK = 32768, MAX_SET = 512;
-struct GradSet {
+// The tensors of one launch travel in the kernel's parameters: up to MAX of
+// them, 16 (0.6 KB of parameters) or 512 (18 KB).  A tensor is cut into
+// chunks of CHUNK bytes, which the launch's blocks take in turn; first[i] is
+// the number of chunks before tensor i.
+constexpr unsigned CHUNK = 32768, FEW = 16, MANY = 512;
+template <unsigned MAX> struct GradSet {
   unsigned count, chunks;
-  unsigned first[MAX_SET];
-  tc_gradient of[MAX_SET];
+  unsigned first[MAX];
+  tc_gradient of[MAX];
 };
 
-__device__ __forceinline__ unsigned find(const GradSet &set, unsigned chunk) {
+template <unsigned MAX> __device__ __forceinline__ unsigned find(const GradSet<MAX> &set, unsigned chunk) {
   unsigned low = 0, high = set.count - 1;
   while (low < high) {
     const unsigned mid = (low + high + 1) / 2;
@@ -76,9 +77,15 @@ __device__ __forceinline__ double block_sum(double v, double *room) {
   return v;
 }
 
-// Each block's sum of squares, at partial[slot + block].
-__global__ void __launch_bounds__(256) square_sums(const __grid_constant__ GradSet set, double *partial, unsigned slot) {
-  __shared__ double room[8];
+// Each block's sum of squares, at partial[slot + block].  Of the `total`
+// blocks of the call's launches the last to finish adds up all of them, in
+// their order, and sets the ticket back to zero.
+template <unsigned MAX>
+__global__ void __launch_bounds__(256) square_sums(const __grid_constant__ GradSet<MAX> set, double *partial, unsigned slot,
+                                                   unsigned total, int *ticket, float *norm) {
+  __shared__ double room[2][8];
+  __shared__ bool last;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // clip_set, which waits for the norm
   double sum = 0.0;
   for (unsigned c = blockIdx.x; c < set.chunks; c += gridDim.x) {
     const unsigned i = find(set, c);
@@ -103,19 +110,32 @@ __global__ void __launch_bounds__(256) square_sums(const __grid_constant__ GradS
           });
     });
   }
-  sum = block_sum(sum, room);
-  if (threadIdx.x == 0) partial[slot + blockIdx.x] = sum;
+  sum = block_sum(sum, room[0]);
+  if (threadIdx.x == 0) {
+    partial[slot + blockIdx.x] = sum;
+    __threadfence();
+    last = unsigned(atomicAdd(ticket, 1)) == total - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  sum = 0.0;
+  for (unsigned i = threadIdx.x; i < total; i += blockDim.x) sum += __ldcg(partial + i);
+  sum = block_sum(sum, room[1]);
+  if (threadIdx.x == 0) {
+    *norm = float(sqrt(sum));
+    *ticket = 0;
+  }
 }
 
-__global__ void __launch_bounds__(256) norm_of(const double *partial, unsigned n, float *norm) {
-  __shared__ double room[8];
-  double sum = 0.0;
-  for (unsigned i = threadIdx.x; i < n; i += blockDim.x) sum += partial[i];
-  sum = block_sum(sum, room);
-  if (threadIdx.x == 0) *norm = float(sqrt(sum));
-}
+// The norm of no gradients.
+__global__ void zero_norm(float *norm) { *norm = 0.0f; }
 
-__global__ void __launch_bounds__(256) clip_set(const __grid_constant__ GradSet set, const float *norm, float limit) {
+// The chunks from the last to the first: the last ones read for the norm are
+// still in L2.
+template <unsigned MAX>
+__global__ void __launch_bounds__(256) clip_set(const __grid_constant__ GradSet<MAX> set, const float *norm, float limit) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const float n = *norm;
   // a norm of zero clips nothing; a NaN carries on
   const float by = n <= limit ? 1.0f : limit / n;
@@ -134,7 +154,14 @@ __global__ void __launch_bounds__(256) clip_set(const __grid_constant__ GradSet 
           [&](size_t at, Run<S, V> r) {
 #pragma unroll
             for (unsigned j = 0; j < V; ++j) r.e[j] = T::store(T::load(r.e[j]) * by);
-            if (whole) store_run<S, V>(out + at, r);
+            if (whole) {
+              union {
+                uint4 w;
+                Run<S, V> r;
+              } u;
+              u.r = r;
+              __stcs(reinterpret_cast<uint4 *>(out + at), u.w);
+            }
             else
 #pragma unroll
               for (unsigned j = 0; j < V; ++j) out[at + j] = r.e[j];
@@ -156,13 +183,13 @@ int check_list(const char *what, const tc_gradient *grads, size_t count, bool ou
 }
 
 // The list in sets of one launch each: f(set).
-template <class F> int in_sets(const tc_gradient *grads, size_t count, F &&f) {
-  GradSet set;
+template <unsigned MAX, class F> int in_sets(const tc_gradient *grads, size_t count, F &&f) {
+  GradSet<MAX> set;
   set.count = set.chunks = 0;
   for (size_t i = 0; i < count; ++i) {
     if (grads[i].n == 0) continue;
     const size_t per = CHUNK / dtype_bytes(grads[i].dtype), chunks = (grads[i].n + per - 1) / per;
-    if (set.count == MAX_SET || set.chunks + chunks > 0x7fffffffu) {
+    if (set.count == MAX || set.chunks + chunks > 0x7fffffffu) {
       if (set.count)
         if (int st = f(set)) return st;
       set.count = set.chunks = 0;
@@ -172,6 +199,45 @@ template <class F> int in_sets(const tc_gradient *grads, size_t count, F &&f) {
     set.chunks += unsigned(chunks);
   }
   return set.count ? f(set) : TC_OK;
+}
+
+template <unsigned MAX> int norm_run(const tc_gradient *grads, size_t count, float *norm, cudaStream_t on) {
+  const unsigned blocks = unsigned(sm_count()) * 8;
+  unsigned total = 0;
+  in_sets<MAX>(grads, count, [&](const GradSet<MAX> &set) {
+    total += std::min(blocks, set.chunks);
+    return int(TC_OK);
+  });
+  if (total == 0) {
+    zero_norm<<<1, 1, 0, on>>>(norm);
+    return check_launch("grad norm");
+  }
+  void *room = nullptr;
+  if (int st = scratch(size_t(total) * sizeof(double), &room, on)) return st;
+  int *ticket = nullptr;
+  if (int st = counters(1, &ticket, on)) return st;
+  unsigned slot = 0;
+  return in_sets<MAX>(grads, count, [&](const GradSet<MAX> &set) -> int {
+    const unsigned grid = std::min(blocks, set.chunks);
+    square_sums<MAX><<<grid, 256, 0, on>>>(set, static_cast<double *>(room), slot, total, ticket, norm);
+    slot += grid;
+    return check_launch("grad norm");
+  });
+}
+
+template <unsigned MAX> int clip_run(const tc_gradient *grads, size_t count, const float *norm, float limit, cudaStream_t on) {
+  return in_sets<MAX>(grads, count, [&](const GradSet<MAX> &set) -> int {
+    cudaLaunchAttribute early{};  // beside the norm's last blocks
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(std::min(unsigned(sm_count()) * 8, set.chunks));
+    config.blockDim = dim3(256);
+    config.stream = on;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&config, clip_set<MAX>, set, norm, limit), "clip grads");
+  });
 }
 
 }  // namespace
@@ -184,34 +250,15 @@ extern "C" {
 int tc_grad_norm(const tc_gradient *grads, size_t count, float *norm, void *stream) {
   if (int st = check_list("grad norm", grads, count, false)) return st;
   if (!norm) return fail(TC_EINVAL, "grad norm: null pointer");
-  cudaStream_t on = as_stream(stream);
-  const unsigned blocks = unsigned(sm_count()) * 8;
-  size_t sets = 0;
-  if (int st = in_sets(grads, count, [&](const GradSet &) { return ++sets, int(TC_OK); })) return st;
-  void *room = nullptr;
-  if (int st = scratch(std::max<size_t>(1, sets) * blocks * sizeof(double), &room, on)) return st;
-  double *partial = static_cast<double *>(room);
-  unsigned filled = 0;
-  if (int st = in_sets(grads, count, [&](const GradSet &set) -> int {
-        const unsigned grid = std::min(blocks, set.chunks);
-        square_sums<<<grid, 256, 0, on>>>(set, partial, filled);
-        filled += grid;
-        return check_launch("grad norm");
-      }))
-    return st;
-  norm_of<<<1, 256, 0, on>>>(partial, filled, norm);
-  return check_launch("grad norm");
+  return count <= FEW ? norm_run<FEW>(grads, count, norm, as_stream(stream)) : norm_run<MANY>(grads, count, norm, as_stream(stream));
 }
 
 int tc_clip_grads(const tc_gradient *grads, size_t count, const float *norm, double limit, void *stream) {
   if (int st = check_list("clip grads", grads, count, true)) return st;
   if (!norm) return fail(TC_EINVAL, "clip grads: null pointer");
   if (!(limit >= 0.0)) return fail(TC_EINVAL, "clip grads: limit %g", limit);
-  return in_sets(grads, count, [&](const GradSet &set) -> int {
-    const unsigned grid = std::min(unsigned(sm_count()) * 8, set.chunks);
-    clip_set<<<grid, 256, 0, as_stream(stream)>>>(set, norm, float(limit));
-    return check_launch("clip grads");
-  });
+  return count <= FEW ? clip_run<FEW>(grads, count, norm, float(limit), as_stream(stream))
+                      : clip_run<MANY>(grads, count, norm, float(limit), as_stream(stream));
 }
 
 }  // extern "C"
