@@ -35,27 +35,31 @@ template <unsigned MAX> __device__ __forceinline__ unsigned find(const GradSet<M
   return low;
 }
 
-// Elements [begin, end) of a tensor's chunk: single ones up to the first
-// 16-byte boundary, runs of 16 bytes, single ones after them.
+// The elements of a tensor before its first 128-byte line (at most n): the
+// first chunk has them beside its own, so that every chunk's runs of 16 bytes
+// fill whole lines, wherever the tensor starts.
+__host__ __device__ __forceinline__ size_t before_line(const void *p, size_t n, size_t bytes) {
+  const size_t k = (128 - reinterpret_cast<uintptr_t>(p) % 128) % 128 / bytes;
+  return k < n ? k : n;
+}
+// one(index, element) and many(index, run) for this thread's share of a chunk.
 template <class S, class One, class Many>
 __device__ __forceinline__ void walk_chunk(const S *p, size_t n, unsigned chunk, One &&one, Many &&many) {
   constexpr unsigned V = 16 / sizeof(S), PER = CHUNK / sizeof(S);
-  const size_t begin = size_t(chunk) * PER;
-  const unsigned len = unsigned(min(size_t(PER), n - begin));
-  const S *at = p + begin;
-  const unsigned off = unsigned(reinterpret_cast<uintptr_t>(at) & 15) / unsigned(sizeof(S));
-  const unsigned head = min(len, (V - off) % V), runs = (len - head) / V, after = head + runs * V;
+  const size_t lead = before_line(p, n, sizeof(S)), begin = lead + size_t(chunk) * PER;
   const unsigned t = threadIdx.x;
-  if (t < head) one(begin + t, at[t]);
+  if (chunk == 0 && t < lead) one(t, p[t]);
+  const unsigned len = unsigned(min(size_t(PER), n - begin)), runs = len / V, after = runs * V;
+  const S *at = p + begin;
   unsigned i = t;
   for (; i + 3 * blockDim.x < runs; i += 4 * blockDim.x) {
     Run<S, V> r[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) r[u] = load_run<S, V>(at + head + size_t(i + u * blockDim.x) * V);
+    for (int u = 0; u < 4; ++u) r[u] = load_run<S, V>(at + size_t(i + u * blockDim.x) * V);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) many(begin + head + size_t(i + u * blockDim.x) * V, r[u]);
+    for (int u = 0; u < 4; ++u) many(begin + size_t(i + u * blockDim.x) * V, r[u]);
   }
-  for (; i < runs; i += blockDim.x) many(begin + head + size_t(i) * V, load_run<S, V>(at + head + size_t(i) * V));
+  for (; i < runs; i += blockDim.x) many(begin + size_t(i) * V, load_run<S, V>(at + size_t(i) * V));
   if (t < len - after) one(begin + after + t, at[after + t]);
 }
 
@@ -188,7 +192,8 @@ template <unsigned MAX, class F> int in_sets(const tc_gradient *grads, size_t co
   set.count = set.chunks = 0;
   for (size_t i = 0; i < count; ++i) {
     if (grads[i].n == 0) continue;
-    const size_t per = CHUNK / dtype_bytes(grads[i].dtype), chunks = (grads[i].n + per - 1) / per;
+    const size_t bytes = dtype_bytes(grads[i].dtype), per = CHUNK / bytes;
+    const size_t chunks = std::max<size_t>(1, (grads[i].n - before_line(grads[i].g, grads[i].n, bytes) + per - 1) / per);
     if (set.count == MAX || set.chunks + chunks > 0x7fffffffu) {
       if (set.count)
         if (int st = f(set)) return st;
