@@ -637,6 +637,15 @@ int tc_tape_matmul(tc_tape *tape, uint32_t a, uint32_t b, uint32_t *out);
 /* The sum of every element, a one-element var; backward fills (MatrixVar::
  * sum, tape/mod.rs:1286-1296). */
 int tc_tape_sum(tc_tape *tape, uint32_t a, uint32_t *out);
+/* Layer norm over the last axis (tc_layer_norm), weight and bias vars of one
+ * value per column; backward through tc_layer_norm_backward.  The reference's
+ * tape has no counterpart of this rule and the next. */
+int tc_tape_layer_norm(tc_tape *tape, uint32_t a, uint32_t weight, uint32_t bias, double eps, uint32_t *out);
+/* -scale times the sum of the log probabilities (tc_token_logprobs) of
+ * `tokens`, one per row of the logits' last axis, read in place until the
+ * tape is destroyed; a one-element var (scale = 1 / tokens gives the mean
+ * loss).  Backward through tc_token_logprobs_backward. */
+int tc_tape_token_loss(tc_tape *tape, uint32_t logits, const uint32_t *tokens, double scale, uint32_t *out);
 /* A var's value: device pointer, rank and shape (shape may be NULL). */
 int tc_tape_value(tc_tape *tape, uint32_t var, const void **dev, uint32_t *rank, size_t *shape);
 /* Clear every adjoint, seed the one-element `var` with one and apply every

@@ -191,6 +191,8 @@ SIGNATURES = {
     "tc_tape_sum_axes": [_p, _u32, _u32, _u32p, _i, _i, _d, _u32p],
     "tc_tape_matmul": [_p, _u32, _u32, _u32p],
     "tc_tape_sum": [_p, _u32, _u32p],
+    "tc_tape_layer_norm": [_p, _u32, _u32, _u32, _d, _u32p],
+    "tc_tape_token_loss": [_p, _u32, _p, _d, _u32p],
     "tc_tape_value": [_p, _u32, C.POINTER(_p), _u32p, _szp],
     "tc_tape_backward": [_p, _u32],
     "tc_tape_adjoint": [_p, _u32, C.POINTER(_p)],

@@ -70,6 +70,12 @@ int peer_adam_run(int dtype, const PeerAdam &x, int resumed, double rate, double
 void *peer_buffer_remote(tc_peer_buffer *buf, int rank);
 int comm_barrier(tc_comm *comm);
 
+// out (one element of `dtype`) = -scale * sum(logprobs), in f32 and in an
+// order that the count gives; and the logprobs' gradient from that of out:
+// grad = -scale * adjoint (logprob.cu).
+int token_loss_value(int dtype, const float *logprobs, size_t rows, double scale, void *out, cudaStream_t stream);
+int token_loss_seed(int dtype, const void *adjoint, size_t rows, double scale, float *grad, cudaStream_t stream);
+
 // The means and sums of squared deviations (in the element type) of the
 // slices of `input` folded over `axes`, in as few passes as the layout
 // allows (reduce.cu).

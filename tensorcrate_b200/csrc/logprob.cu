@@ -982,6 +982,19 @@ template <class T, bool ENT> __global__ void __launch_bounds__(512) token_slope(
   }
 }
 
+// -scale * the sum of the logprobs, by one block.
+template <class T> __global__ void __launch_bounds__(1024) loss_value(const float *logprobs, size_t rows, float scale, typename T::S *out) {
+  __shared__ float room[32];
+  float sum = 0.0f;
+  for (size_t r = threadIdx.x; r < rows; r += blockDim.x) sum += logprobs[r];
+  sum = block_sum(sum, room);
+  if (threadIdx.x == 0) *out = T::store(-scale * sum);
+}
+template <class T> __global__ void __launch_bounds__(256) loss_seed(const typename T::S *adjoint, size_t rows, float scale, float *grad) {
+  const float g = -scale * T::load(*adjoint);
+  for (size_t r = size_t(blockIdx.x) * blockDim.x + threadIdx.x; r < rows; r += size_t(gridDim.x) * blockDim.x) grad[r] = g;
+}
+
 int check(const char *what, size_t rows, size_t vocab, size_t stride, const char *name) {
   if (vocab == 0) return fail(TC_EINVAL, "%s: a vocabulary of no tokens", what);
   if (vocab >= TC_NO_TOKEN) return fail(TC_ERANGE, "%s: a vocabulary of %zu tokens", what, vocab);
@@ -1090,6 +1103,22 @@ template <class T, bool ENT> int backward(const TokenArgs &a, cudaStream_t strea
 }
 
 }  // namespace
+
+int token_loss_value(int dtype, const float *logprobs, size_t rows, double scale, void *out, cudaStream_t stream) {
+  return with_real(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    loss_value<T><<<1, 1024, 0, stream>>>(logprobs, rows, float(scale), static_cast<typename T::S *>(out));
+    return check_launch("token loss");
+  });
+}
+int token_loss_seed(int dtype, const void *adjoint, size_t rows, double scale, float *grad, cudaStream_t stream) {
+  if (rows == 0) return TC_OK;
+  return with_real(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    loss_seed<T><<<grid_for(rows, 256), 256, 0, stream>>>(static_cast<const typename T::S *>(adjoint), rows, float(scale), grad);
+    return check_launch("token loss");
+  });
+}
 }  // namespace tc
 
 using namespace tc;

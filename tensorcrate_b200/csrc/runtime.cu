@@ -326,7 +326,8 @@ const char *tc_build_info(void) {
   return "tensorcrate_b200 0.1 sm_100a: strided copy/assemble/write, elementwise, strided binary, "
          "axis reduce, arg reduce, tcgen05 bf16/f16 GEMM and 3xTF32 f32 GEMM with epilogues, gemv, "
          "Adam/SGD, fused programs (statistics, sums, GEMM epilogues), analytic unary and dual, power, "
-         "prefix sum, sort, correlation, pad, flip, moments, distributions, NCCL and NVLink peer stores";
+         "prefix sum, sort, correlation, pad, flip, moments, distributions, layer norm, token log "
+         "probabilities, gradient clipping, NCCL and NVLink peer stores";
 }
 
 int tc_set_device(int device) { return check_cuda(cudaSetDevice(device), "cudaSetDevice"); }

@@ -20,14 +20,17 @@
 //     tape/tensor.rs:317-323, 581-620; matmul as MatrixVar::matmul
 //     (tape/mod.rs:1190-1216: Ā += C̄·Bᵀ, B̄ += Aᵀ·C̄, accumulated into the
 //     current adjoint or zeros); sum as MatrixVar::sum (tape/mod.rs:1286-1296,
-//     the adjoint filled with the output's adjoint).
+//     the adjoint filled with the output's adjoint);
+//   - layer norm and the token loss, which the reference's tape has not: nodes
+//     over tc_layer_norm and tc_token_logprobs that keep the forward pass's
+//     statistics for their backward calls.
 #include <vector>
 
 #include "common.cuh"
 
 namespace {
 
-enum Kind { LEAF, BINARY, RELU, SCALE, SUM_AXES, MATMUL, SUM };
+enum Kind { LEAF, BINARY, RELU, SCALE, SUM_AXES, MATMUL, SUM, LAYER_NORM, TOKEN_LOSS };
 
 struct Node {
   Kind kind = LEAF;
@@ -39,8 +42,20 @@ struct Node {
   uint32_t a = 0, b = 0;
   std::vector<uint32_t> axes;
   bool mean = false;
-  double factor = 0;  // scale's factor, mean's share (values of the element type)
+  double factor = 0;  // scale's factor, mean's share (values of the element type); the token loss's scale
+  // layer norm: a the input, b the weight, c the bias; token loss: a the logits
+  uint32_t c = 0;
+  void *statistics = nullptr;  // owned, f32
+  const uint32_t *tokens = nullptr;
 };
+
+// The last axis, and what is before it.
+size_t cols_of(const std::vector<size_t> &shape) { return shape.back(); }
+size_t rows_of(const std::vector<size_t> &shape) {
+  size_t n = 1;
+  for (size_t i = 0; i + 1 < shape.size(); ++i) n *= shape[i];
+  return n;
+}
 
 size_t count_of(const std::vector<size_t> &shape) {
   size_t n = 1;
@@ -67,6 +82,7 @@ namespace {
   } while (0)
 
 int alloc(tc_tape *t, size_t n, void **out) { return tc_malloc_async(out, std::max<size_t>(n * t->esz, 16), t->stream); }
+int alloc_bytes(tc_tape *t, size_t bytes, void **out) { return tc_malloc_async(out, std::max<size_t>(bytes, 16), t->stream); }
 void release(tc_tape *t, void *p) {
   if (p) tc_free_async(p, t->stream);
 }
@@ -262,6 +278,31 @@ int propagate(tc_tape *t, uint32_t i) {
       TRY(spread(t, g, std::vector<size_t>(p.shape.size(), 1), p.shape, &d));
       return accumulate(t, p, d);
     }
+    case LAYER_NORM: {
+      Node &x = t->nodes[n.a], &w = t->nodes[n.b], &b = t->nodes[n.c];
+      const size_t rows = rows_of(n.shape), cols = cols_of(n.shape);
+      void *dx = nullptr, *dw = nullptr, *db = nullptr;
+      TRY(alloc(t, rows * cols, &dx));
+      TRY(alloc(t, cols, &dw));
+      TRY(alloc(t, cols, &db));
+      TRY(tc_layer_norm_backward(t->dtype, t->dtype, rows, cols, g, cols, x.value, cols, static_cast<float *>(n.statistics),
+                                 w.value, dx, cols, dw, db, t->stream));
+      TRY(accumulate(t, x, dx));
+      TRY(accumulate(t, w, dw));
+      return accumulate(t, b, db);
+    }
+    case TOKEN_LOSS: {
+      Node &x = t->nodes[n.a];
+      const size_t rows = rows_of(x.shape), cols = cols_of(x.shape);
+      void *seed = nullptr, *dx = nullptr;
+      TRY(alloc_bytes(t, rows * sizeof(float), &seed));
+      TRY(token_loss_seed(t->dtype, g, rows, n.factor, static_cast<float *>(seed), t->stream));
+      TRY(alloc(t, rows * cols, &dx));
+      TRY(tc_token_logprobs_backward(t->dtype, rows, cols, x.value, cols, n.tokens, static_cast<float *>(n.statistics), nullptr,
+                                     static_cast<float *>(seed), nullptr, dx, cols, t->stream));
+      release(t, seed);
+      return accumulate(t, x, dx);
+    }
     default:
       return TC_OK;
   }
@@ -287,6 +328,7 @@ int tc_tape_destroy(tc_tape *t) {
   for (Node &n : t->nodes) {
     if (n.owned) release(t, n.value);
     release(t, n.adjoint);
+    release(t, n.statistics);
   }
   delete t;
   return TC_OK;
@@ -403,6 +445,66 @@ int tc_tape_sum(tc_tape *t, uint32_t a, uint32_t *out) {
   TRY(alloc(t, 1, &n.value));
   n.owned = true;
   TRY(tc_vector_reduce(t->dtype, TC_SUM, t->nodes[a].value, count_of(t->nodes[a].shape), n.value, t->stream));
+  return push(t, std::move(n), out);
+}
+
+int tc_tape_layer_norm(tc_tape *t, uint32_t a, uint32_t weight, uint32_t bias, double eps, uint32_t *out) {
+  TRY(check_var(t, a));
+  TRY(check_var(t, weight));
+  TRY(check_var(t, bias));
+  const std::vector<size_t> &shape = t->nodes[a].shape;
+  if (shape.empty() || cols_of(shape) == 0) return fail(TC_EINVAL, "tape_layer_norm: rows of no elements");
+  const size_t cols = cols_of(shape), rows = rows_of(shape);
+  if (count_of(t->nodes[weight].shape) != cols || count_of(t->nodes[bias].shape) != cols)
+    return fail(TC_EINVAL, "tape_layer_norm: weight and bias do not hold one value for each of %zu columns", cols);
+  if (!(eps >= 0.0)) return fail(TC_EINVAL, "tape_layer_norm: eps %g", eps);
+  Node n;
+  n.kind = LAYER_NORM;
+  n.a = a;
+  n.b = weight;
+  n.c = bias;
+  n.shape = shape;
+  n.owned = true;
+  int st = alloc(t, count_of(shape), &n.value);
+  if (!st) st = alloc_bytes(t, 2 * rows * sizeof(float), &n.statistics);
+  if (!st)
+    st = tc_layer_norm(t->dtype, t->dtype, rows, cols, t->nodes[a].value, cols, t->nodes[weight].value, t->nodes[bias].value, eps,
+                       n.value, cols, static_cast<float *>(n.statistics), t->stream);
+  if (st) {
+    release(t, n.value);
+    release(t, n.statistics);
+    return st;
+  }
+  return push(t, std::move(n), out);
+}
+
+int tc_tape_token_loss(tc_tape *t, uint32_t logits, const uint32_t *tokens, double scale, uint32_t *out) {
+  TRY(check_var(t, logits));
+  const std::vector<size_t> &shape = t->nodes[logits].shape;
+  if (shape.empty() || cols_of(shape) == 0) return fail(TC_EINVAL, "tape_token_loss: a vocabulary of no tokens");
+  const size_t vocab = cols_of(shape), rows = rows_of(shape);
+  if (rows && !tokens) return fail(TC_EINVAL, "tape_token_loss: null tokens");
+  Node n;
+  n.kind = TOKEN_LOSS;
+  n.a = logits;
+  n.shape = {1};
+  n.owned = true;
+  n.factor = scale;
+  n.tokens = tokens;
+  void *logprobs = nullptr;
+  int st = alloc(t, 1, &n.value);
+  if (!st) st = alloc_bytes(t, 2 * rows * sizeof(float), &n.statistics);
+  if (!st) st = alloc_bytes(t, rows * sizeof(float), &logprobs);
+  if (!st)
+    st = tc_token_logprobs(t->dtype, rows, vocab, t->nodes[logits].value, vocab, tokens, static_cast<float *>(logprobs), nullptr,
+                           static_cast<float *>(n.statistics), 0, nullptr, nullptr, t->stream);
+  if (!st) st = token_loss_value(t->dtype, static_cast<float *>(logprobs), rows, scale, n.value, t->stream);
+  release(t, logprobs);
+  if (st) {
+    release(t, n.value);
+    release(t, n.statistics);
+    return st;
+  }
   return push(t, std::move(n), out);
 }
 

@@ -12,14 +12,31 @@ TcError.  Nothing waits for the device.
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 from typing import Sequence
 
 from . import _native as N
-from .cuda import CudaStorage, Tensor, TensorView, _stream
+from .cuda import ELEM, CudaStorage, Tensor, TensorView, _stream
 
 NO_TOKEN = N.NO_TOKEN
 MAX_TOP = N.MAX_TOP
+
+
+_BYTES = {name: nbytes for name, (_, nbytes) in ELEM.items()}
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    return getattr(N.lib(), name)
+
+
+def _run(name: str, stream, *args) -> None:
+    """N.call with the stream last, its entry point looked up once: small
+    calls cost what their checks do."""
+    status = _entry(name)(*args, stream if type(stream) is int else _stream(stream))
+    if status:
+        N.check(name, status)
 
 
 def _matrix(what: str, x, dtype: str | None = None) -> tuple[int, int, int, int]:
@@ -32,48 +49,51 @@ def _matrix(what: str, x, dtype: str | None = None) -> tuple[int, int, int, int]
     cols, rows = shape[-1], 1
     for e in shape[:-1]:
         rows *= e
-    if not isinstance(x, TensorView):
+    if type(x) is Tensor:
         return storage.ptr, rows, cols, cols
     strides = x.strides
     if cols > 1 and strides[-1] != 1:
         raise ValueError(f"{what}: the last axis steps by {strides[-1]}, call contiguous() first")
-    stride, step = cols, None
-    for e, s in zip(reversed(shape[:-1]), reversed(strides[:-1])):
-        if e == 1:
-            continue
-        if step is None:
-            stride = s
-        elif s != step:
-            raise ValueError(f"{what}: the leading axes {shape[:-1]} do not step as one, call contiguous() first")
-        step = s * e
+    if len(shape) == 2:
+        stride = strides[0] if rows > 1 else cols
+    else:
+        stride, step = cols, None
+        for e, s in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+            if e == 1:
+                continue
+            if step is None:
+                stride = s
+            elif s != step:
+                raise ValueError(f"{what}: the leading axes {shape[:-1]} do not step as one, call contiguous() first")
+            step = s * e
     if rows and cols:
         reach = x.offset + (rows - 1) * stride + cols
         if reach > storage.len:
             raise ValueError(f"{what}: reaches element {reach}, past {storage.len} elements")
-    return storage.ptr + x.offset * storage.elem_bytes, rows, cols, stride
+    return storage.ptr + x.offset * _BYTES[storage.dtype], rows, cols, stride
 
 
 def _vector(what: str, x, n: int, dtypes: Sequence[str]) -> int | None:
     """The address of x's n contiguous elements; None for None."""
     if x is None:
         return None
-    storage, offset = x, 0
-    if not isinstance(x, CudaStorage):
-        storage = x.storage
-        if isinstance(x, TensorView):
-            if not x.is_contiguous():
-                raise ValueError(f"{what}: not contiguous")
-            offset = x.offset
-        held = 1
-        for e in x.shape:
-            held *= e
+    kind, offset = type(x), 0
+    if kind is CudaStorage:
+        storage, held = x, x.len
     else:
-        held = x.len
+        storage, shape = x.storage, x.shape
+        held = 1
+        for e in shape:
+            held *= e
+        if kind is TensorView:
+            offset = x.offset
+            if shape and (len(shape) > 1 or x.strides[0] != 1) and not x.is_contiguous():
+                raise ValueError(f"{what}: not contiguous")
     if storage.dtype not in dtypes:
         raise ValueError(f"{what}: element type {storage.dtype}, expected {' or '.join(dtypes)}")
     if held != n or offset + n > storage.len:
         raise ValueError(f"{what}: {held} elements, expected {n}")
-    return storage.ptr + offset * storage.elem_bytes
+    return storage.ptr + offset * _BYTES[storage.dtype]
 
 
 def _like(x, shape, dtype: str) -> Tensor:
@@ -84,7 +104,7 @@ def _like(x, shape, dtype: str) -> Tensor:
 
 
 def _same_shape(what: str, x, y) -> None:
-    if list(x.shape) != list(y.shape):
+    if x.shape != y.shape and list(x.shape) != list(y.shape):
         raise ValueError(f"{what}: shapes {list(x.shape)} and {list(y.shape)} differ")
 
 
@@ -111,13 +131,12 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None, statistic
     if statistics is None:
         statistics = _like(x, [rows, 2], "f32")
     st = _vector("layer_norm: statistics", statistics, 2 * rows, ("f32",))
-    N.call("tc_layer_norm", N.DTYPES[dtype], N.DTYPES[kind], rows, cols, ptr, stride, w, b, eps, yptr, ystride, st,
-           _stream(stream))
+    _run("tc_layer_norm", stream, N.DTYPES[dtype], N.DTYPES[kind], rows, cols, ptr, stride, w, b, eps, yptr, ystride, st)
     return out, statistics
 
 
 def _dtype(x) -> str | None:
-    return None if x is None else x.dtype
+    return None if x is None else x.dtype if type(x) is CudaStorage else x.storage.dtype
 
 
 def layer_norm_backward(grad, x, statistics, weight=None, out=None, grad_weight=None, grad_bias=None, stream=None):
@@ -142,8 +161,8 @@ def layer_norm_backward(grad, x, statistics, weight=None, out=None, grad_weight=
         grad_bias = _like(x, [cols], kind)
     gw = _vector("layer_norm_backward: grad_weight", grad_weight, cols, (kind,))
     gb = _vector("layer_norm_backward: grad_bias", grad_bias, cols, (kind,))
-    N.call("tc_layer_norm_backward", N.DTYPES[dtype], N.DTYPES[kind], rows, cols, gptr, gstride, ptr, stride, st, w,
-           optr, ostride, gw, gb, _stream(stream))
+    _run("tc_layer_norm_backward", stream, N.DTYPES[dtype], N.DTYPES[kind], rows, cols, gptr, gstride, ptr, stride, st, w,
+           optr, ostride, gw, gb)
     return out, grad_weight, grad_bias
 
 
@@ -171,9 +190,9 @@ def _fresh(rows: int, tokens, entropy: bool, top: int) -> TokenLogprobs:
 
 
 def _results(what: str, out: TokenLogprobs, rows: int) -> tuple:
-    return (_vector(f"{what}: logprobs", out.logprobs, rows, ("f32",)),
-            _vector(f"{what}: entropy", out.entropy, rows, ("f32",)),
-            _vector(f"{what}: statistics", out.statistics, 2 * rows, ("f32",)))
+    return (_vector(what + ": logprobs", out.logprobs, rows, ("f32",)),
+            _vector(what + ": entropy", out.entropy, rows, ("f32",)),
+            _vector(what + ": statistics", out.statistics, 2 * rows, ("f32",)))
 
 
 def token_logprobs(logits, tokens=None, top: int = 0, entropy: bool = True, out: TokenLogprobs | None = None,
@@ -194,8 +213,8 @@ def token_logprobs(logits, tokens=None, top: int = 0, entropy: bool = True, out:
     lp, ent, st = _results("token_logprobs", out, rows)
     tt = _vector("token_logprobs: top_tokens", out.top_tokens, rows * top, ("u32",))
     tl = _vector("token_logprobs: top_logprobs", out.top_logprobs, rows * top, ("f32",))
-    N.call("tc_token_logprobs", N.DTYPES[logits.storage.dtype], rows, vocab, ptr, stride,
-           tok, lp, ent, st, top, tt, tl, _stream(stream))
+    _run("tc_token_logprobs", stream, N.DTYPES[logits.storage.dtype], rows, vocab, ptr, stride,
+           tok, lp, ent, st, top, tt, tl)
     return out
 
 
@@ -207,7 +226,7 @@ def token_logprobs_backward(logits, tokens, statistics, grad_logprobs=None, entr
     logits."""
     ptr, rows, vocab, stride = _matrix("token_logprobs_backward: logits", logits)
     dtype = logits.storage.dtype
-    each = [_vector(f"token_logprobs_backward: {name}", v, rows, (kind,))
+    each = [_vector("token_logprobs_backward: " + name, v, rows, (kind,))
             for name, v, kind in (("tokens", tokens, "u32"), ("entropy", entropy, "f32"),
                                   ("grad_logprobs", grad_logprobs, "f32"), ("grad_entropy", grad_entropy, "f32"))]
     st = _vector("token_logprobs_backward: statistics", statistics, 2 * rows, ("f32",))
@@ -216,8 +235,8 @@ def token_logprobs_backward(logits, tokens, statistics, grad_logprobs=None, entr
     else:
         _same_shape("token_logprobs_backward", logits, out)
     optr, _, _, ostride = _matrix("token_logprobs_backward: out", out, dtype)
-    N.call("tc_token_logprobs_backward", N.DTYPES[dtype], rows, vocab, ptr, stride, each[0], st, each[1], each[2],
-           each[3], optr, ostride, _stream(stream))
+    _run("tc_token_logprobs_backward", stream, N.DTYPES[dtype], rows, vocab, ptr, stride, each[0], st, each[1], each[2],
+           each[3], optr, ostride)
     return out
 
 
@@ -242,7 +261,7 @@ def token_loss(logits, tokens, grad_logprobs, grad_entropy=None, out: TokenLogpr
         _same_shape("token_loss", logits, grad)
     gptr, _, _, gstride = _matrix("token_loss: grad", grad, dtype)
     lp, ent, st = _results("token_loss", out, rows)
-    N.call("tc_token_loss", N.DTYPES[dtype], rows, vocab, ptr, stride, *given, lp, ent, st, gptr, gstride, _stream(stream))
+    _run("tc_token_loss", stream, N.DTYPES[dtype], rows, vocab, ptr, stride, *given, lp, ent, st, gptr, gstride)
     return out, grad
 
 
@@ -278,7 +297,7 @@ def grad_norm(grads, out=None, stream=None):
     grads = _list(grads)
     if out is None:
         out = _like(None, [1], "f32")
-    N.call("tc_grad_norm", grads.entries, grads.count, _vector("grad_norm: out", out, 1, ("f32",)), _stream(stream))
+    _run("tc_grad_norm", stream, grads.entries, grads.count, _vector("grad_norm: out", out, 1, ("f32",)))
     return out
 
 
@@ -286,5 +305,4 @@ def clip_grads(grads, norm, limit: float, stream=None) -> None:
     """Every gradient times min(1, limit / norm), norm a device f32 (grad_norm's,
     or one combined over ranks)."""
     grads = _list(grads)
-    N.call("tc_clip_grads", grads.entries, grads.count, _vector("clip_grads: norm", norm, 1, ("f32",)), float(limit),
-           _stream(stream))
+    _run("tc_clip_grads", stream, grads.entries, grads.count, _vector("clip_grads: norm", norm, 1, ("f32",)), float(limit))

@@ -62,6 +62,17 @@ class Tape:
     def sum(self, a: int) -> int:
         return self._out("tc_tape_sum", a)
 
+    def layer_norm(self, a: int, weight: int, bias: int, eps: float = 1e-5) -> int:
+        return self._out("tc_tape_layer_norm", a, weight, bias, float(eps))
+
+    def token_loss(self, logits: int, tokens: CudaStorage, scale: float) -> int:
+        """-scale * sum of the tokens' log probabilities (u32, one per row)."""
+        rows = int(np.prod(self.shape(logits)[:-1], dtype=np.int64))
+        if tokens.dtype != "u32" or tokens.len != rows:
+            raise ValueError(f"token_loss: {tokens.len} tokens of {tokens.dtype}, expected {rows} of u32")
+        self._keep.append(tokens)
+        return self._out("tc_tape_token_loss", logits, tokens.ptr, float(scale))
+
     def shape(self, v: int) -> list[int]:
         rank = C.c_uint32()
         shape = (C.c_size_t * N.MAX_RANK)()
@@ -84,6 +95,22 @@ class Tape:
 
     def backward(self, v: int) -> None:
         N.call("tc_tape_backward", self.handle, v)
+
+    def _storage(self, ptr, v: int) -> CudaStorage | None:
+        shape = self.shape(v)
+        return CudaStorage(self.dtype, int(np.prod(shape, dtype=np.int64)), ptr=ptr) if ptr else None
+
+    def value_storage(self, v: int) -> CudaStorage:
+        """A var's value on the device, the tape's."""
+        p = C.c_void_p()
+        N.call("tc_tape_value", self.handle, v, C.byref(p), None, None)
+        return self._storage(p.value, v)
+
+    def grad_storage(self, v: int) -> CudaStorage | None:
+        """The adjoint on the device, the tape's until its next backward."""
+        p = C.c_void_p()
+        N.call("tc_tape_adjoint", self.handle, v, C.byref(p))
+        return self._storage(p.value, v)
 
     def grad(self, v: int):
         """The adjoint after backward, or None when nothing reached v."""
