@@ -488,9 +488,12 @@ __device__ __forceinline__ void top_of_row(const typename T::S *row, const Cut<T
   } else {
     if (t < c.head) keep(t, T::load(row[t]));
     if (t < c.tail) keep(c.after + t, T::load(row[c.after + t]));
-    for (unsigned h = warp; h < holders; h += warps)
-      for (size_t i = room.holder[h] + size_t(t & 31) * threads; i < c.runs; i += size_t(threads) * 32)
-        keep_run(unsigned(i), load(unsigned(i)));
+    // the holders' runs dealt out to all threads
+    const unsigned all = holders * ((c.runs + threads - 1) / threads);
+    for (unsigned x = t; x < all; x += threads) {
+      const unsigned i = room.holder[x % holders] + x / holders * threads;
+      if (i < c.runs) keep_run(i, load(i));
+    }
   }
   sync();
   const unsigned count = room.count;
