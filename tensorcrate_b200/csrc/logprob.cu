@@ -567,8 +567,8 @@ template <bool ENT, bool WILD> __device__ __forceinline__ F2 slope_of_pair(const
   const F2 c = add2(pair(fmaxf(z.x, -1e30f), fmaxf(z.y, -1e30f)), pair(g.entropy, g.entropy));
   return mul2(p, fma2(c, pair(-g.v, -g.v), pair(-g.u, -g.u)));
 }
-// The gradient at the run that begins at element `at`.
-template <class T, bool ENT, bool WILD> __device__ __forceinline__ uint4 slope_run(const Slope &g, const Bits<T> &r, unsigned at) {
+// The gradient at a run, but for the token's own term.
+template <class T, bool ENT, bool WILD> __device__ __forceinline__ uint4 slope_run(const Slope &g, const Bits<T> &r) {
   using S = typename T::S;
   constexpr unsigned V = Cut<T>::V;
   F2 d[V / 2];
@@ -584,14 +584,26 @@ template <class T, bool ENT, bool WILD> __device__ __forceinline__ uint4 slope_r
   } else {
     out.w = make_uint4(narrow2<T>(d[0]), narrow2<T>(d[1]), narrow2<T>(d[2]), narrow2<T>(d[3]));
   }
-  if (g.token - at < V) {
-    const S special = T::store(slope_at<ENT>(g, r.at(g.token - at), g.token));
-#pragma unroll
-    for (unsigned j = 0; j < V; ++j)
-      if (at + j == g.token) out.e[j] = special;
-  }
   return out.w;
 }
+// The token's own element of the gradient: the thread that writes its run
+// stores it after that run.
+template <class T> struct Own {
+  unsigned run = ~0u;  // the token's, where this thread has it
+  typename T::S value;
+  template <bool ENT>
+  __device__ __forceinline__ void find(const typename T::S *row, const Cut<T> &c, const Slope &g, unsigned t, unsigned threads) {
+    if (g.token < c.body || g.token - c.body >= c.runs * Cut<T>::V) return;
+    const unsigned i = (g.token - c.body) / Cut<T>::V;
+    if (i % threads != t) return;
+    run = i;
+    value = T::store(slope_at<ENT>(g, T::load(row[g.token]), g.token));
+  }
+  // After the runs from i, `threads` apart, U of them.
+  __device__ __forceinline__ void after(unsigned i, unsigned span, typename T::S *to, unsigned token) const {
+    if (run - i < span) to[token] = value;
+  }
+};
 // A run of the gradient's row, whole where it lies on the grid as the logits do.
 template <class T> __device__ __forceinline__ void put_run(typename T::S *to, uint4 w, bool whole) {
   using S = typename T::S;
@@ -629,6 +641,8 @@ __device__ __forceinline__ void write_slope(const typename T::S *row, typename T
     write_zeros<T>(to, c, t, threads, whole);
     return;
   }
+  Own<T> own;
+  own.template find<ENT>(row, c, g, t, threads);
   auto write = [&](auto wild) {
     walk<T>(
         row, c, t, threads, from_row<T>(row, c), [&](unsigned at, S e) { to[at] = T::store(slope_at<ENT>(g, T::load(e), at)); },
@@ -637,8 +651,9 @@ __device__ __forceinline__ void write_slope(const typename T::S *row, typename T
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             const unsigned at = c.body + (i + u * threads) * V;
-            put_run<T>(to + at, slope_run<T, ENT, decltype(wild)::value>(g, r[u], at), whole);
+            put_run<T>(to + at, slope_run<T, ENT, decltype(wild)::value>(g, r[u]), whole);
           }
+          own.after(i, U * threads, to, g.token);
         });
   };
   if (g.wild) write(std::true_type{});
@@ -773,11 +788,14 @@ template <class T, bool ENT, int EXTRA, int U> __global__ void __launch_bounds__
         for (int u = 0; u < U; ++u) {
           const unsigned i = lane + 32 * u, at = c.body + i * V;
           if (i < c.runs)
-            put_run<T>(to + at, none ? make_uint4(0, 0, 0, 0) : slope_run<T, ENT, decltype(wild)::value>(g, bits[u], at), whole);
+            put_run<T>(to + at, none ? make_uint4(0, 0, 0, 0) : slope_run<T, ENT, decltype(wild)::value>(g, bits[u]), whole);
         }
       };
+      Own<T> own;
+      if (!none) own.template find<ENT>(row, c, g, lane, 32);
       if (g.wild) write(std::true_type{});
       else write(std::false_type{});
+      if (own.run != ~0u) to[g.token] = own.value;
       if (single != ~0u) to[single] = none ? S(0) : T::store(slope_at<ENT>(g, extra, single));
     }
   }
@@ -843,8 +861,10 @@ template <class T> struct Ahead {
   }
 };
 
-// Larger ones: a block a row, or a cluster's blocks, each a part of it.
-template <class T, bool ENT, int EXTRA> __global__ void __launch_bounds__(256, 6) token_rows(const TokenArgs a) {
+// Larger ones: a block a row, or a cluster's blocks, each a part of it.  (The
+// top tokens' code spills with the registers of six blocks: 2048x50257 bf16
+// takes 77 us with six, 69 with five.)
+template <class T, bool ENT, int EXTRA> __global__ void __launch_bounds__(256, EXTRA == TOP ? 5 : 6) token_rows(const TokenArgs a) {
   using S = typename T::S;
   constexpr unsigned V = Cut<T>::V;
   __shared__ Slots joint;
@@ -929,6 +949,8 @@ template <class T, bool ENT> __global__ void __launch_bounds__(256, 3) token_los
       if (t < c.head) to[t] = T::store(slope_at<ENT>(s, T::load(row[t]), t));
       if (t < c.tail) to[c.after + t] = T::store(slope_at<ENT>(s, T::load(row[c.after + t]), c.after + t));
     }
+    Own<T> own;
+    if (!none) own.template find<ENT>(row, c, s, t, threads);
     auto write = [&](auto wild) {
       for (unsigned g = 0; g < groups; ++g) {
         if (!none)
@@ -937,8 +959,9 @@ template <class T, bool ENT> __global__ void __launch_bounds__(256, 3) token_los
 #pragma unroll
             for (int u = 0; u < U; ++u) {
               const unsigned at = c.body + (i + u * threads) * V;
-              put_run<T>(to + at, slope_run<T, ENT, decltype(wild)::value>(s, bits[u], at), whole);
+              put_run<T>(to + at, slope_run<T, ENT, decltype(wild)::value>(s, bits[u]), whole);
             }
+            own.after(i, U * threads, to, s.token);
           });
         ring.fetch();
       }
