@@ -107,8 +107,8 @@ template <class T, int U> __device__ __forceinline__ float largest(const Bits<T>
 constexpr float TAME = 1024.0f, LN2 = 0.6931471805599453f;
 __device__ __forceinline__ bool tame(float m) { return fabsf(m) <= TAME; }
 
-// A pair of elements no lower than -1e37 (-65504): weightless wherever m is
-// tame, and finite.  NaNs stay.
+// The elements, none of them lower than -1e37 (f16: -65504): weightless there
+// wherever m is tame, and finite, so that e a is 0.  NaNs stay.
 template <class T> __device__ __forceinline__ Bits<T> lifted(Bits<T> r) {
   if constexpr (T::code == TC_F32) {
     auto up = [](uint32_t w) {
@@ -212,8 +212,8 @@ template <class T, bool ENT> struct Running {
 };
 
 // A row's elements, or the part of them that one of `of` (a power of two)
-// blocks has, as runs
-// of 16 aligned bytes with the few single elements before and after them.
+// blocks has, as runs of 16 aligned bytes with the few single elements before
+// and after them.
 template <class T> struct Cut {
   using S = typename T::S;
   static constexpr unsigned V = 16 / sizeof(S);
@@ -724,7 +724,9 @@ template <class T> __device__ __forceinline__ float logit_of(const typename T::S
 enum Extra { NOTHING = 0, TOP = 1, GRADIENT = 2 };
 
 // Small vocabularies: a warp holds a row, U runs a lane.  The row is read
-// once, whatever is asked for but the top tokens' second look.
+// once, whatever is asked for but the top tokens' second look.  Bound by
+// issue: 65536x1000 bf16 with entropy in 34 us (floor 20), with 5 top tokens
+// in 116; the loss of 65536x1024 in 59 (floor 42).
 template <class T, bool ENT, int EXTRA, int U> __global__ void __launch_bounds__(256) token_small(const TokenArgs a) {
   using S = typename T::S;
   constexpr unsigned V = Cut<T>::V;
@@ -861,9 +863,14 @@ template <class T> struct Ahead {
   }
 };
 
-// Larger ones: a block a row, or a cluster's blocks, each a part of it.  (The
-// top tokens' code spills with the registers of six blocks: 2048x50257 bf16
-// takes 77 us with six, 69 with five.)
+// Larger ones: a block a row, or a cluster's blocks, each a part of it.  Four
+// 16-byte loads a thread and 1536 threads an SM cover HBM's latency (the same
+// rows copied ahead through shared memory took 58 us for 56).  8192x32768 bf16
+// with entropy in 93 us, 5.8 TB/s; 2048x50257 in 44 us, where 2.3 rounds of
+// blocks begin and end together.  With top tokens the steps between the row's
+// barriers, not HBM, take the time: 66 us with 8 of them, some rows masked to
+// nothing.  (Their code spills with the registers of six blocks an SM: 77 us;
+// five are kept.)
 template <class T, bool ENT, int EXTRA> __global__ void __launch_bounds__(256, EXTRA == TOP ? 5 : 6) token_rows(const TokenArgs a) {
   using S = typename T::S;
   constexpr unsigned V = Cut<T>::V;
@@ -918,7 +925,7 @@ template <class T, bool ENT, int EXTRA> __global__ void __launch_bounds__(256, E
 
 // The loss of rows that a block's shared memory holds: a row stays in its
 // slots until its gradient is written from there, and the next one follows it
-// group by group.
+// group by group.  16384x8192 bf16 in 108 us, 5.0 TB/s (138 us read twice).
 template <class T, bool ENT> __global__ void __launch_bounds__(256, 3) token_loss_held(const TokenArgs a, unsigned groups) {
   using S = typename T::S;
   constexpr unsigned V = Cut<T>::V;
@@ -972,7 +979,10 @@ template <class T, bool ENT> __global__ void __launch_bounds__(256, 3) token_los
 }
 
 // Larger rows, and few: the blocks of a cluster share a row, and the second
-// pass reads it from L2, which the parts of all resident blocks leave room in.
+// pass reads it from L2, which the parts of all resident blocks leave room in
+// (2.1 GB of HBM traffic at 4096x131072 bf16, where blocks of whole rows made
+// it 3.1).  420 us, 5.1 TB/s: the two passes' exponentials keep the special
+// function unit 60% busy between the row's barriers.
 template <class T, bool ENT> __global__ void __launch_bounds__(256, 4) token_loss_twice(const TokenArgs a) {
   using S = typename T::S;
   __shared__ Slots joint;
@@ -995,7 +1005,8 @@ template <class T, bool ENT> __global__ void __launch_bounds__(256, 4) token_los
 }
 
 // The gradient alone, from the statistics that the forward call left, by
-// blocks or (`apart`) by warps of a row each.
+// blocks or (`apart`) by warps of a row each.  Bound by HBM: 4096x32768 f32
+// with entropy in 168 us, 6.4 TB/s.
 template <class T, bool ENT> __global__ void __launch_bounds__(512) token_slope(const TokenArgs a, bool apart) {
   using S = typename T::S;
   const unsigned threads = apart ? 32 : blockDim.x, each = blockDim.x / threads;
@@ -1072,10 +1083,6 @@ unsigned parts_for(size_t rows, size_t runs, unsigned threads, size_t slots) {
 // takes 411 us in four parts, 462 in two, 476 in one; 4096x50257 (6282) 175
 // in one, 181 in two.
 constexpr size_t PART_RUNS = 6400;
-template <class K> int allow_shared(K kernel, size_t most) {
-  return check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most)), "token logprobs");
-}
-
 // A warp a row up to 8 runs a lane; 2 or 4 where those do.
 template <class T, bool ENT, int EXTRA> int small(const char *what, const TokenArgs &a, cudaStream_t stream) {
   const unsigned grid = unsigned(std::min<size_t>((a.rows + 7) / 8, size_t(sm_count()) * 64));
@@ -1107,8 +1114,8 @@ template <class T, bool ENT> int loss(const TokenArgs &a, cudaStream_t stream) {
   if (runs <= 16 * size_t(threads) && a.rows > size_t(sm_count())) {
     auto kernel = token_loss_held<T, ENT>;
     const size_t groups = (runs + 4 * threads - 1) / (4 * threads), shared = groups * 4 * 16 * threads;
-    static const int allowed = allow_shared(kernel, 16 * 16 * 256);
-    if (allowed) return allowed;
+    static std::atomic<uint64_t> allowed{0};
+    if (int st = allow_shared("token loss", reinterpret_cast<const void *>(kernel), 16 * 16 * 256, allowed)) return st;
     const unsigned grid = unsigned(std::min<size_t>(a.rows, resident(kernel, threads, shared)));
     kernel<<<grid, threads, shared, stream>>>(a, unsigned(groups));
     return check_launch("token loss");

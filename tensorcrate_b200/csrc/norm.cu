@@ -15,10 +15,11 @@
 namespace tc {
 namespace {
 
-// A row's elements stay in the registers of the threads that share it, so x
-// is read once for both of the variance's passes.  Access k of thread t
-// covers the E elements from (t + k * threads) * E: neighbours read
-// neighbouring addresses.
+// A row's elements stay in the registers of the threads that share it (a
+// warp's up to 1024 columns, else a block's), so x is read once for both of
+// the variance's passes.  Access k of thread t covers the E elements from (t
+// + k * threads) * E: neighbours read neighbouring addresses.  Bound by HBM:
+// 32768x1024 f32 in 48 us, 5.6 TB/s (43 us of it the kernel's).
 template <class T, class P, int E, int K, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_rows(const typename T::S *x, size_t x_stride,
                                                   const typename P::S *__restrict__ w,
@@ -78,8 +79,8 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_rows(const typename T:
   }
 }
 
-// Rows too wide for the registers of one block: a block reads its row three
-// times, the second and third from L2.
+// Rows of more than 16384 columns: a block reads its row three times, the
+// second and third from L2.
 template <class T, class P>
 __global__ void __launch_bounds__(1024) norm_rows_wide(const typename T::S *x, size_t x_stride,
                                                        const typename P::S *__restrict__ w,
@@ -126,13 +127,18 @@ __global__ void __launch_bounds__(1024) norm_rows_wide(const typename T::S *x, s
 // full width; a granule that holds one valid byte can be read whole); E
 // elements at a time are taken from there, E > 1 only for rows on the grid.
 // One barrier a turn publishes the rows' sums, the next turn's data and the
-// stage to be filled again.
+// stage to be filled again.  A turn's elements are read from the ring twice
+// (kept in registers across the barrier, with the sums, they spill).  Two rows
+// a turn share its barrier, its waits and its shuffles: one row leaves a block
+// of 16 warps, all in step, with too little between them.
 //
-// HOLD: the turn's elements stay in registers across the barrier, as they
-// are stored, so its stage is filled again at once; else they are read again
-// and the stage is filled after the next barrier.  Two rows a turn share its
-// barrier, its waits and its shuffles: one row leaves a block of 16 warps,
-// all in step, with too little between them.
+// What bounds it: HBM until about 2000 columns; for wider rows the one block
+// that an SM's registers hold, 16 warps that issue half of the time and
+// whose integer pipe (the widening of two reads of two tensors, addresses) is
+// two thirds busy.  16384x8192 bf16, 805 MB: 170 us for this kernel and 182
+// us a call, 4.4 TB/s (one row a turn: 186 us a call; 1024 threads of 8
+// columns each spill: 289 us; rows through registers without the ring: 263
+// us); 2048x4096 bf16 24.6 us, 4099x1001 f16 18.0 us a call.
 struct NormGrad {
   const void *g, *x, *w;
   size_t g_stride, x_stride, dx_stride, rows;
@@ -189,7 +195,7 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
   using PS = typename P::S;
   using Row = Held<T, E, K>;
   constexpr int N = Row::N, STEP = Row::STEP;
-  constexpr bool HOLD = false, KEEP_W = K * E <= 16;
+  constexpr bool KEEP_W = K * E <= 16;  // wider rows read the weights again
   constexpr int GRANULES = K * E * int(sizeof(S)) / 16 + (E == 1);  // a thread's, of a row
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float room[2][64];
@@ -233,7 +239,7 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
     copy_commit();
   };
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  constexpr unsigned AHEAD = HOLD ? DEPTH : DEPTH - 1;  // turns in the ring at a turn's start
+  constexpr unsigned AHEAD = DEPTH - 1;  // turns in the ring at a turn's start
 #pragma unroll
   for (unsigned d = 0; d < AHEAD; ++d) fill(d);
 
@@ -317,8 +323,8 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
       if (row + r < a.rows) next[r] = a.statistics[row + r];
     copy_wait<AHEAD - 2>();  // this thread's part of the next turn
     sync();
-    // every thread is past this turn's data (HOLD), or past the last turn's
-    fill(HOLD ? stage : stage == 0 ? DEPTH - 1 : stage - 1);
+    // every thread is past the last turn, whose stage comes before this one
+    fill(stage == 0 ? DEPTH - 1 : stage - 1);
     v = ((lane & 7) < warps ? at[warp0 + (lane & 7)] : 0.0f) + ((lane & 7) + 8 < warps ? at[warp0 + (lane & 7) + 8] : 0.0f);
 #pragma unroll
     for (int o = 4; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -329,10 +335,8 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
         const float c1 = __shfl_sync(0xffffffffu, v, 16 * r) * st[r].y, c2 = __shfl_sync(0xffffffffu, v, 16 * r + 8) * st[r].y;
         if (R > 1 && row - every * R + r >= a.rows) break;
         const F2 mean = pair(-st[r].x, -st[r].x), rstd = pair(st[r].y, st[r].y), k1 = pair(c1, c1), k2 = pair(c2, c2);
-        if (!HOLD) {
-          xr[r].load(held_at(2 * r, x_here + r * x_step), t, threads, cols);
-          gr[r].load(held_at(2 * r + 1, g_here + r * g_step), t, threads, cols);
-        }
+        xr[r].load(held_at(2 * r, x_here + r * x_step), t, threads, cols);
+        gr[r].load(held_at(2 * r + 1, g_here + r * g_step), t, threads, cols);
 #pragma unroll
         for (int i = 0; i < N; i += STEP) {
           F2 out[STEP];
@@ -591,8 +595,8 @@ int tc_layer_norm_backward(int dtype, int param_dtype, size_t rows, size_t cols,
     auto launch = [&](auto e, auto k, auto two) -> int {
       constexpr int E = decltype(e)::value, K = decltype(k)::value, R = decltype(two)::value;
       auto kernel = norm_grad_rows<T, P, E, K, R>;
-      static const cudaError_t allowed = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RING);
-      if (int st = check_cuda(allowed, "layer norm backward")) return st;
+      static std::atomic<uint64_t> allowed{0};
+      if (int st = allow_shared("layer norm backward", reinterpret_cast<const void *>(kernel), RING, allowed)) return st;
       NormGrad a{grad, x, weight, grad_stride, x_stride, grad_x_stride, rows, stats, grad_x, nullptr, unsigned(cols), 0, unsigned(slot)};
       const unsigned n = unsigned((cols + E - 1) / E);
       a.threads = ((n + K - 1) / K + 31) / 32 * 32;

@@ -3,6 +3,8 @@
 // access, and sums over a warp and over a block.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace tc {
@@ -142,6 +144,18 @@ __device__ __forceinline__ float block_sum(float v, float *room) {
   if (lane == 0) room[threadIdx.x >> 5] = v;
   __syncthreads();
   return warp_sum(lane < warps ? room[lane] : 0.0f);
+}
+
+// Let `kernel` have up to `bytes` of dynamic shared memory on the current
+// device; `done` remembers the devices that were told.
+inline int allow_shared(const char *what, const void *kernel, size_t bytes, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  if (int st = check_cuda(cudaGetDevice(&dev), what)) return st;
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return TC_OK;
+  if (int st = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)), what)) return st;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return TC_OK;
 }
 
 // Whether runs of E elements of `bytes` each can be moved whole from rows
