@@ -79,6 +79,140 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_rows(const typename T:
   }
 }
 
+// The same for 16-bit rows on the 16-byte grid, where the weights (often f32)
+// would be read again for each row at several times its bytes: blocks that
+// stay, of groups of `threads` threads.  A group takes a turn of R
+// neighbouring rows at a time and its threads own the same K * E columns of
+// every row, whose weights and biases they keep in registers; the next
+// turn's rows are loaded before this one's are used.
+struct NormTurns {
+  const void *x, *w, *b;
+  void *y;
+  size_t x_stride, y_stride, rows;
+  float2 *statistics;
+  float eps;
+  unsigned cols, threads;
+};
+template <class T, class P, int K, int R, int MOST, int BLOCKS>
+__global__ void __launch_bounds__(MOST, BLOCKS) norm_turns(const NormTurns a) {
+  using S = typename T::S;
+  using PS = typename P::S;
+  constexpr int E = 8, N = K * 4;  // elements of an access, pairs of a row
+  __shared__ float room[2][2][32];
+  const unsigned threads = a.threads, groups = blockDim.x / threads, cols = a.cols;
+  const unsigned group = threadIdx.x / threads, t = threadIdx.x - group * threads;
+  const unsigned lane = threadIdx.x & 31, warps = threads >> 5, warp0 = group * warps;
+  const size_t every = size_t(gridDim.x) * groups * R;
+  size_t row = (size_t(blockIdx.x) * groups + group) * R;
+  auto column = [&](int k) { return (t + k * threads) * E; };
+  uint4 next[R][K];
+  auto fetch = [&](size_t at) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        next[r][k] = make_uint4(0, 0, 0, 0);
+        if (at + r < a.rows && column(k) < cols)
+          next[r][k] = *reinterpret_cast<const uint4 *>(static_cast<const S *>(a.x) + (at + r) * a.x_stride + column(k));
+      }
+  };
+  fetch(row);
+  F2 w[N], b[N];
+  auto keep = [&](const void *from, float none, F2 *into) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float v[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = none;
+      if (from && column(k) < cols) load_wide<P, E>(static_cast<const PS *>(from) + column(k), v);
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) into[k * 4 + j] = pair(v[2 * j], v[2 * j + 1]);
+    }
+  };
+  keep(a.w, 1.0f, w);
+  keep(a.b, 0.0f, b);
+  const float share = 1.0f / float(cols);
+  // A value of each of the R rows, added over the group's threads.
+  auto add_up = [&](float (&v)[R], int which) {
+    float s;
+    if constexpr (R == 2) {  // lanes 0 to 15 add up the first row's, 16 to 31 the second's
+      s = lane < 16 ? v[0] : v[1];
+      s += __shfl_xor_sync(0xffffffffu, lane < 16 ? v[1] : v[0], 16);
+    } else {
+      s = v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
+    }
+#pragma unroll
+    for (int o = 8; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (warps > 1) {
+      float *at = room[which][R == 2 ? lane >> 4 : 0];
+      if ((lane & 15) == 0) at[threadIdx.x >> 5] = s;
+      __barrier_sync_count(group + 1, threads);
+      s = 0.0f;
+      for (unsigned i = lane & 15; i < warps; i += 16) s += at[warp0 + i];
+#pragma unroll
+      for (int o = 8; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] = __shfl_sync(0xffffffffu, s, 16 * r);
+  };
+  for (; row < a.rows; row += every) {
+    uint4 raw[R][K];
+    float mean[R], rstd[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int k = 0; k < K; ++k) raw[r][k] = next[r][k];
+    fetch(row + every);
+    auto pair_at = [&](int r, int i) {
+      const uint4 q = raw[r][i / 4];
+      return widen2<T>(i % 4 == 0 ? q.x : i % 4 == 1 ? q.y : i % 4 == 2 ? q.z : q.w);
+    };
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      F2 s = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) s = add2(s, pair_at(r, i));
+      const float2 p = split(s);
+      mean[r] = p.x + p.y;
+    }
+    add_up(mean, 0);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mean[r] *= share;
+      const F2 less = pair(-mean[r], -mean[r]);
+      F2 s = 0;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (column(k) < cols)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const F2 d = add2(pair_at(r, k * 4 + j), less);
+            s = fma2(d, d, s);
+          }
+      const float2 p = split(s);
+      rstd[r] = p.x + p.y;
+    }
+    add_up(rstd, 1);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      rstd[r] = __frsqrt_rn(rstd[r] * share + a.eps);
+      if (row + r >= a.rows) break;
+      if (t == 0 && a.statistics) a.statistics[row + r] = make_float2(mean[r], rstd[r]);
+      const F2 less = pair(-mean[r], -mean[r]), scale = pair(rstd[r], rstd[r]);
+      S *to = static_cast<S *>(a.y) + (row + r) * a.y_stride;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (column(k) < cols) {
+          F2 out[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            out[j] = fma2(mul2(add2(pair_at(r, k * 4 + j), less), scale), w[k * 4 + j], b[k * 4 + j]);
+          store_pairs<T>(to + column(k), out);
+        }
+    }
+  }
+}
+
 // Rows of more than 16384 columns: a block reads its row three times, the
 // second and third from L2.
 template <class T, class P>
@@ -539,7 +673,30 @@ int tc_layer_norm(int dtype, int param_dtype, size_t rows, size_t cols, const vo
       }
       return check_launch("layer norm");
     };
-    if (cols <= 16 * 1024) return whole ? launch(std::integral_constant<int, V>{}) : launch(std::integral_constant<int, 1>{});
+    if constexpr (sizeof(S) == 2) {
+      if (whole && cols <= 16 * 1024) {
+        // 16 columns a thread where 512 of them hold a row, else 32
+        auto turns = [&](auto kernel, unsigned most_threads, unsigned of_thread, unsigned r) -> int {
+          const unsigned threads = unsigned((cols + of_thread - 1) / of_thread + 31) / 32 * 32;
+          const NormTurns a{x, weight, bias, y, x_stride, y_stride, rows, stats, float(eps), unsigned(cols), threads};
+          const unsigned groups = std::max(1u, most_threads / threads);
+          int blocks = 0;
+          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, int(groups * threads), 0);
+          const size_t all = (rows + r - 1) / r;
+          const unsigned grid = unsigned(std::min<size_t>((all + groups - 1) / groups, size_t(std::max(1, blocks)) * size_t(sm_count())));
+          kernel<<<grid, groups * threads, 0, on>>>(a);
+          return check_launch("layer norm");
+        };
+        if (cols <= 16 * 256) return turns(norm_turns<T, P, 2, 2, 256, 2>, 256, 16, 2);
+        if (cols <= 16 * 512) return turns(norm_turns<T, P, 2, 2, 512, 1>, 512, 16, 2);
+        return turns(norm_turns<T, P, 4, 1, 512, 1>, 512, 32, 1);
+      }
+    }
+    if (cols <= 16 * 1024) {
+      if constexpr (sizeof(S) == 4)
+        if (whole) return launch(std::integral_constant<int, V>{});
+      return launch(std::integral_constant<int, 1>{});
+    }
     norm_rows_wide<T, P><<<most, 1024, 0, on>>>(xs, x_stride, ws, bs, float(eps), ys, y_stride, stats, rows, cols);
     return check_launch("layer norm");
   });
