@@ -18,8 +18,10 @@ namespace {
 // A row's elements stay in the registers of the threads that share it (a
 // warp's up to 1024 columns, else a block's), so x is read once for both of
 // the variance's passes.  Access k of thread t covers the E elements from (t
-// + k * threads) * E: neighbours read neighbouring addresses.  Bound by HBM:
-// 32768x1024 f32 in 48 us, 5.6 TB/s (43 us of it the kernel's).
+// + k * threads) * E: neighbours read neighbouring addresses.  f32 rows are
+// bound by HBM: 32768x1024 in 48 us, 5.6 TB/s (43 us of it the kernel's); rows
+// off the 16-byte grid (E = 1) by their single accesses, 65536x1001 bf16 in
+// 108 us, 38% of the floor.
 template <class T, class P, int E, int K, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_rows(const typename T::S *x, size_t x_stride,
                                                   const typename P::S *__restrict__ w,
@@ -84,7 +86,11 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_rows(const typename T:
 // stay, of groups of `threads` threads.  A group takes a turn of R
 // neighbouring rows at a time and its threads own the same K * E columns of
 // every row, whose weights and biases they keep in registers; the next
-// turn's rows are loaded before this one's are used.
+// turn's rows are loaded before this one's are used.  16384x8192 bf16 with f32
+// weights in 109 us, 4.9 TB/s (169 us by blocks of a row each that read the
+// weights again); 32768x4096 103, 5.2 TB/s (156); 65536x1024 54 (60).  Single
+// elements of rows off the grid gain nothing by it (65536x1001: 152 us for
+// 108), they stay with norm_rows.
 struct NormTurns {
   const void *x, *w, *b;
   void *y;
@@ -266,10 +272,11 @@ __global__ void __launch_bounds__(1024) norm_rows_wide(const typename T::S *x, s
 // a turn share its barrier, its waits and its shuffles: one row leaves a block
 // of 16 warps, all in step, with too little between them.
 //
-// What bounds it: HBM until about 2000 columns; for wider rows the one block
-// that an SM's registers hold, 16 warps that issue half of the time and
-// whose integer pipe (the widening of two reads of two tensors, addresses) is
-// two thirds busy.  16384x8192 bf16, 805 MB: 170 us for this kernel and 182
+// What bounds it: the one block that an SM's registers hold, 16 warps that
+// issue half of the time (of the HBM floor: f32 rows 93% up to 4096 columns,
+// 16-bit rows 78 to 82% there and 73% at 8192); past 8192 columns the sums
+// spill (28% at 16384), and off the 16-byte grid the single 2-byte accesses
+// take over (47% at 1001 columns).  16384x8192 bf16, 805 MB: 170 us for this kernel and 182
 // us a call, 4.4 TB/s (one row a turn: 186 us a call; 1024 threads of 8
 // columns each spill: 289 us; rows through registers without the ring: 263
 // us); 2048x4096 bf16 24.6 us, 4099x1001 f16 18.0 us a call.
