@@ -255,28 +255,6 @@ template <class T> __device__ __forceinline__ auto from_row(const typename T::S 
   return [p](unsigned i) { return Bits<T>{p[i]}; };
 }
 
-// The blocks of a cluster share a row: this block's part, and how many there
-// are (1 without a cluster).
-__device__ __forceinline__ unsigned cluster_part() {
-  unsigned v;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(v));
-  return v;
-}
-__device__ __forceinline__ unsigned cluster_parts() {
-  unsigned v;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(v));
-  return v;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Store to the same variable of block `part`.
-template <class V> __device__ __forceinline__ void store_at(V *own, unsigned part, V v) {
-  uint32_t to;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(uint32_t(__cvta_generic_to_shared(own))), "r"(part));
-  if constexpr (sizeof(V) == 4) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to), "r"(__float_as_uint(v)) : "memory");
-  else asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(to), "l"(v) : "memory");
-}
 // The sums of a row over the warps of the cluster's blocks (at most 64), the
 // same in every thread: each warp's go to every block.  The slots of two rows
 // in turn: a warp that is ahead stores a row's sums while another still reads
@@ -1043,24 +1021,6 @@ int check(const char *what, size_t rows, size_t vocab, size_t stride, const char
   return TC_OK;
 }
 bool off_grid(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
-
-// Launch `kernel` in clusters of `parts` blocks.
-template <class... A>
-int launch(const char *what, void (*kernel)(A...), size_t clusters, unsigned parts, unsigned threads, size_t shared,
-           cudaStream_t stream, std::common_type_t<A>... args) {
-  cudaLaunchAttribute cluster{};
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = parts;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3(unsigned(clusters * parts));
-  config.blockDim = dim3(threads);
-  config.dynamicSmemBytes = shared;
-  config.stream = stream;
-  config.attrs = &cluster;
-  config.numAttrs = parts > 1 ? 1 : 0;
-  return check_cuda(cudaLaunchKernelEx(&config, kernel, args...), what);
-}
 
 // Blocks of `kernel` that the GPU holds at once.
 template <class K> size_t resident(K kernel, unsigned threads, size_t shared) {

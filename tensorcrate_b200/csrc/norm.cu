@@ -260,6 +260,10 @@ __global__ void __launch_bounds__(1024) norm_rows_wide(const typename T::S *x, s
 // sums stay in registers until the block adds its groups' and writes them to
 // its row of `partial` (w's sums, then b's).
 //
+// WIDE: rows too wide for one block's registers are shared by the blocks of a
+// cluster, each with `width` columns (and one group): the barrier is then the
+// cluster's, and each warp's sums go to every block.
+//
 // The rows come through a ring of DEPTH turns in shared memory, filled
 // asynchronously: HBM is not waited for once the ring runs, whatever few
 // threads the columns' sums leave room for.  A row is copied as the aligned
@@ -274,9 +278,10 @@ __global__ void __launch_bounds__(1024) norm_rows_wide(const typename T::S *x, s
 //
 // What bounds it: the one block that an SM's registers hold, 16 warps that
 // issue half of the time (of the HBM floor: f32 rows 93% up to 4096 columns,
-// 16-bit rows 78 to 82% there and 73% at 8192); past 8192 columns the sums
-// spill (28% at 16384), and off the 16-byte grid the single 2-byte accesses
-// take over (47% at 1001 columns).  16384x8192 bf16, 805 MB: 170 us for this kernel and 182
+// 16-bit rows 78 to 82% there and 73% at 8192); past 8192 columns the
+// clusters' barriers too (61% at 16384, where 32 columns a thread spilled and
+// reached 28%), and off the 16-byte grid the single 2-byte accesses (47% at
+// 1001 columns).  16384x8192 bf16, 805 MB: 170 us for this kernel and 182
 // us a call, 4.4 TB/s (one row a turn: 186 us a call; 1024 threads of 8
 // columns each spill: 289 us; rows through registers without the ring: 263
 // us); 2048x4096 bf16 24.6 us, 4099x1001 f16 18.0 us a call.
@@ -286,7 +291,7 @@ struct NormGrad {
   const float2 *statistics;
   void *dx;
   float *partial;
-  unsigned cols, threads, slot;  // slot: bytes of one row in the ring
+  unsigned cols, width, threads, slot;  // slot: bytes of a block's part of one row in the ring
 };
 constexpr unsigned RING = 200 * 1024, DEPTH = 3, MAX_GROUPS = 15;  // named barriers 1 to 15
 
@@ -330,28 +335,31 @@ template <class T, int E, int K> struct Held {
   }
 };
 
-template <class T, class P, int E, int K, int R>
+template <class T, class P, int E, int K, int R, bool WIDE>
 __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
   using S = typename T::S;
   using PS = typename P::S;
   using Row = Held<T, E, K>;
   constexpr int N = Row::N, STEP = Row::STEP;
-  constexpr bool KEEP_W = K * E <= 16;  // wider rows read the weights again
   constexpr int GRANULES = K * E * int(sizeof(S)) / 16 + (E == 1);  // a thread's, of a row
   extern __shared__ __align__(16) unsigned char ring[];
-  __shared__ float room[2][64];
-  const unsigned threads = a.threads, groups = blockDim.x / threads, cols = a.cols;
+  __shared__ float room[2][4 * 64];  // four sums of up to 64 warps
+  const unsigned part = WIDE ? cluster_part() : 0, parts = WIDE ? cluster_parts() : 1, base = part * a.width;
+  const unsigned threads = a.threads, groups = blockDim.x / threads, cols = WIDE ? min(a.width, a.cols - base) : a.cols;
   const unsigned group = threadIdx.x / threads, t = threadIdx.x - group * threads;
-  const unsigned lane = threadIdx.x & 31, warps = threads >> 5, warp0 = group * warps;
+  const unsigned lane = threadIdx.x & 31, warps = parts * (threads >> 5), warp0 = group * warps;
   // turn n of this group: rows R (begin + n every), and the next
-  const size_t begin = size_t(blockIdx.x) * groups + group, every = size_t(gridDim.x) * groups;
+  const size_t begin = size_t(blockIdx.x / parts) * groups + group, every = size_t(gridDim.x / parts) * groups;
   const size_t turns = (a.rows + R - 1) / R, count = begin < turns ? (turns - begin + every - 1) / every : 0;
   unsigned char *mine = ring + size_t(group) * DEPTH * 2 * R * a.slot;
   const uint32_t mine32 = uint32_t(__cvta_generic_to_shared(mine));
   auto column = [&](int k) { return (t + k * threads) * E; };
-  auto sync = [&] { __barrier_sync_count(group + 1, threads); };
+  auto sync = [&] {
+    if (WIDE) cluster_sync();
+    else __barrier_sync_count(group + 1, threads);
+  };
   auto row_at = [&](const void *p, size_t stride, size_t row) {
-    return reinterpret_cast<uintptr_t>(static_cast<const S *>(p) + row * stride);
+    return reinterpret_cast<uintptr_t>(static_cast<const S *>(p) + row * stride + base);
   };
 
   // the next turn to be copied
@@ -386,7 +394,7 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
 
   auto load_weight = [&](int i) -> F2 {  // pair i
     if (!a.w) return pair(1.0f, 1.0f);
-    const PS *at = static_cast<const PS *>(a.w);
+    const PS *at = static_cast<const PS *>(a.w) + base;
     if constexpr (E == 1) {
       const unsigned lo = column(2 * i), hi = column(2 * i + 1);
       return pair(lo < cols ? P::load(at[lo]) : 1.0f, hi < cols ? P::load(at[hi]) : 1.0f);
@@ -397,18 +405,17 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
       return pair(P::load(r.e[0]), P::load(r.e[1]));
     }
   };
-  F2 w[KEEP_W ? N : 1], sum_w[N], sum_b[N];
+  F2 w[N], sum_w[N], sum_b[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    if (KEEP_W) w[i] = load_weight(i);
+    w[i] = load_weight(i);
     sum_w[i] = sum_b[i] = 0;
   }
-  auto weight = [&](int i) { return KEEP_W ? w[KEEP_W ? i : 0] : load_weight(i); };
 
-  const float share = 1.0f / float(cols);
+  const float share = 1.0f / float(a.cols);
   size_t row = begin * R;
   uintptr_t x_here = x_next - AHEAD * every * R * x_step, g_here = g_next - AHEAD * every * R * g_step;
-  S *dx = static_cast<S *>(a.dx) + (a.dx ? row * a.dx_stride : 0);
+  S *dx = static_cast<S *>(a.dx) + (a.dx ? row * a.dx_stride + base : 0);
   float2 next[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) next[r] = row + r < a.rows ? a.statistics[row + r] : make_float2(0.0f, 0.0f);
@@ -437,7 +444,7 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
       F2 s1 = 0, s2 = 0;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const F2 h = mul2(add2(xr[r].pair_at(i), mean), rstd), gv = gr[r].pair_at(i), gw = mul2(gv, weight(i));
+        const F2 h = mul2(add2(xr[r].pair_at(i), mean), rstd), gv = gr[r].pair_at(i), gw = mul2(gv, w[i]);
         s1 = add2(s1, gw);
         s2 = fma2(gw, h, s2);
         sum_w[i] = fma2(gv, h, sum_w[i]);
@@ -456,8 +463,12 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
     v += __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 8);
 #pragma unroll
     for (int o = 4; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    float *at = room[turn] + (lane >> 3) * 16;
-    if ((lane & 7) == 0) at[threadIdx.x >> 5] = v;
+    float *at = room[turn] + (lane >> 3) * 64;
+    if ((lane & 7) == 0) {
+      if (!WIDE) at[threadIdx.x >> 5] = v;
+      else
+        for (unsigned p = 0; p < parts; ++p) store_at(at + part * (threads >> 5) + (threadIdx.x >> 5), p, v);
+    }
     row += every * R;
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -467,6 +478,8 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
     // every thread is past the last turn, whose stage comes before this one
     fill(stage == 0 ? DEPTH - 1 : stage - 1);
     v = ((lane & 7) < warps ? at[warp0 + (lane & 7)] : 0.0f) + ((lane & 7) + 8 < warps ? at[warp0 + (lane & 7) + 8] : 0.0f);
+    if (WIDE)
+      for (unsigned i = (lane & 7) + 16; i < warps; i += 8) v += at[i];
 #pragma unroll
     for (int o = 4; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     v *= -share;
@@ -483,7 +496,7 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
           F2 out[STEP];
 #pragma unroll
           for (int j = 0; j < STEP; ++j) {
-            const F2 h = mul2(add2(xr[r].pair_at(i + j), mean), rstd), gw = mul2(gr[r].pair_at(i + j), weight(i + j));
+            const F2 h = mul2(add2(xr[r].pair_at(i + j), mean), rstd), gw = mul2(gr[r].pair_at(i + j), w[i + j]);
             out[j] = fma2(gw, rstd, fma2(h, k2, k1));
           }
           S *to = dx + r * a.dx_stride;
@@ -507,8 +520,8 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
   if (!a.partial) return;
   // the groups' sums: each group's to the ring's memory, then added up in the
   // groups' order by all threads
-  float *out = a.partial + size_t(blockIdx.x) * 2 * cols;
-  float *hold = groups > 1 ? reinterpret_cast<float *>(ring) + size_t(group) * 2 * cols : out;
+  float *out = a.partial + size_t(blockIdx.x / parts) * 2 * a.cols + base;
+  float *hold = groups > 1 ? reinterpret_cast<float *>(ring) + size_t(group) * 2 * a.cols : out;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -516,11 +529,11 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
     const unsigned lo = E == 1 ? column(2 * i) : column(i / STEP) + i % STEP * 2, hi = E == 1 ? column(2 * i + 1) : lo + 1;
     if (lo < cols) {
       hold[lo] = vw.x;
-      hold[cols + lo] = vb.x;
+      hold[a.cols + lo] = vb.x;
     }
     if (hi < cols) {
       hold[hi] = vw.y;
-      hold[cols + hi] = vb.y;
+      hold[a.cols + hi] = vb.y;
     }
   }
   if (groups == 1) return;
@@ -533,7 +546,7 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
   }
 }
 
-// Rows too wide for that: grad_x by blocks that read their row twice ...
+// Rows of more than 32768 columns: grad_x by blocks that read their row twice ...
 template <class T, class P>
 __global__ void __launch_bounds__(1024) norm_grad_wide(const typename T::S *g, size_t g_stride,
                                                        const typename T::S *x, size_t x_stride,
@@ -752,38 +765,45 @@ int tc_layer_norm_backward(int dtype, int param_dtype, size_t rows, size_t cols,
                        runs_fit(x, x_stride, rows, sizeof(S), V) &&
                        (!grad_x || runs_fit(grad_x, grad_x_stride, rows, sizeof(S), V)) &&
                        (!weight || reinterpret_cast<uintptr_t>(weight) % 16 == 0);
-    // Threads own 16 columns where 512 of them hold a row, else 32.  Two rows
-    // a turn where their registers and the ring hold them.
-    const bool narrow = cols <= 16 * 512;
-    const size_t slot = (std::min<size_t>(cols, 16 * 1024) * sizeof(S) + 15) / 16 * 16 + 16;
-    auto launch = [&](auto e, auto k, auto two) -> int {
-      constexpr int E = decltype(e)::value, K = decltype(k)::value, R = decltype(two)::value;
-      auto kernel = norm_grad_rows<T, P, E, K, R>;
-      static std::atomic<uint64_t> allowed{0};
-      if (int st = allow_shared("layer norm backward", reinterpret_cast<const void *>(kernel), RING, allowed)) return st;
-      NormGrad a{grad, x, weight, grad_stride, x_stride, grad_x_stride, rows, stats, grad_x, nullptr, unsigned(cols), 0, unsigned(slot)};
-      const unsigned n = unsigned((cols + E - 1) / E);
-      a.threads = ((n + K - 1) / K + 31) / 32 * 32;
-      // as many groups as the block's threads, its named barriers and the ring
-      // hold, but no more than give every SM a turn
-      const size_t sms = size_t(sm_count()), turns = (rows + R - 1) / R, each = DEPTH * 2 * R * slot;
-      const unsigned groups = unsigned(std::min<size_t>({MAX_GROUPS, 512 / a.threads, RING / each, (turns + sms - 1) / sms}));
-      const unsigned grid = unsigned(std::min<size_t>((turns + groups - 1) / groups, sms));
-      if (sums) {
-        if (int st = room(grid)) return st;
-        a.partial = partial;
-      }
-      kernel<<<grid, groups * a.threads, std::max(groups * each, groups > 1 ? groups * cols * 8 : 0), on>>>(a);
-      return check_launch("layer norm backward");
-    };
-    if (cols <= 16 * 1024 && DEPTH * 2 * slot <= RING) {
+    // A thread owns 16 columns (8 of up to 4096 off the grid), a block those of
+    // 512 threads, a cluster those of at most four blocks.  Two rows a turn
+    // where their registers and the ring hold them.
+    unsigned across = 1;
+    while (across < 4 && cols > 16 * 512 * across) across *= 2;
+    if (cols <= 16 * 512 * across) {
+      auto run = [&](auto e, auto k, auto two, auto wide) -> int {
+        constexpr int E = decltype(e)::value, K = decltype(k)::value, R = decltype(two)::value;
+        auto kernel = norm_grad_rows<T, P, E, K, R, decltype(wide)::value>;
+        static std::atomic<uint64_t> allowed{0};
+        if (int st = allow_shared("layer norm backward", reinterpret_cast<const void *>(kernel), RING, allowed)) return st;
+        const size_t width = ((cols + across - 1) / across + V - 1) / V * V, slot = (width * sizeof(S) + 15) / 16 * 16 + 16;
+        NormGrad a{grad, x, weight, grad_stride, x_stride, grad_x_stride, rows, stats, grad_x, nullptr, unsigned(cols), unsigned(width), 0, unsigned(slot)};
+        a.threads = unsigned((width + K * E - 1) / (K * E) + 31) / 32 * 32;
+        // as many groups as the block's threads, its named barriers and the ring
+        // hold, but no more than give every SM a turn
+        const size_t sms = size_t(sm_count()), turns = (rows + R - 1) / R, each = DEPTH * 2 * R * slot;
+        const unsigned groups = across > 1 ? 1 : unsigned(std::min<size_t>({MAX_GROUPS, 512 / a.threads, RING / each, (turns + sms - 1) / sms}));
+        const unsigned grid = unsigned(std::min<size_t>((turns + groups - 1) / groups, sms / across));
+        if (sums) {
+          if (int st = room(grid)) return st;
+          a.partial = partial;
+        }
+        return tc::launch("layer norm backward", kernel, grid, across, groups * a.threads,
+                          std::max(groups * each, groups > 1 ? groups * cols * 8 : 0), on, a);
+      };
       constexpr int R = sizeof(S) == 2 ? 2 : 1;
+      const std::integral_constant<int, 1> one;
+      const std::integral_constant<int, V> access;
+      const std::integral_constant<int, 16 / V> accesses;
+      const std::integral_constant<int, 8> eight;
+      const std::integral_constant<int, 16> sixteen;
+      const std::integral_constant<int, R> two;
       int st;
-      if (whole && narrow) st = launch(std::integral_constant<int, V>{}, std::integral_constant<int, 16 / V>{}, std::integral_constant<int, R>{});
-      else if (whole) st = launch(std::integral_constant<int, V>{}, std::integral_constant<int, 32 / V>{}, std::integral_constant<int, 1>{});
-      else if (cols <= 8 * 512) st = launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
-      else if (narrow) st = launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
-      else st = launch(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
+      if (whole && across == 1) st = run(access, accesses, two, std::false_type{});
+      else if (whole) st = run(access, accesses, two, std::true_type{});
+      else if (cols <= 8 * 512) st = run(one, eight, one, std::false_type{});
+      else if (across == 1) st = run(one, sixteen, one, std::false_type{});
+      else st = run(one, sixteen, one, std::true_type{});
       if (st) return st;
     } else {
       if (sums) {  // first: grad_x may replace what they read

@@ -94,7 +94,7 @@ def norm_grad64(g, x, w, mean, rstd):
 
 NORM_SHAPES = [(1, 1, 0, 0), (1, 7, 0, 0), (3, 8, 0, 0), (5, 100, 3, 1), (70, 256, 0, 0), (4, 1001, 0, 0), (9, 1024, 0, 0),
                (7, 1032, 8, 8), (130, 1536, 0, 0), (2, 4096, 0, 0), (33, 4099, 0, 0), (3, 5000, 5, 0), (3, 8200, 0, 0),
-               (2, 16384, 0, 0), (3, 16392, 8, 0), (2, 33001, 0, 3), (1, 70000, 0, 0)]
+               (2, 16384, 0, 0), (3, 16392, 8, 0), (5, 9001, 0, 0), (90, 16408, 0, 0), (50, 20003, 0, 1), (2, 33001, 0, 3), (1, 70000, 0, 0)]
 
 
 @pytest.mark.parametrize("params", ["same", "f32", "none"])
