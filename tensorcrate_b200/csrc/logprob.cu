@@ -258,11 +258,14 @@ template <class T> __device__ __forceinline__ auto from_row(const typename T::S 
 // The sums of a row over the warps of the cluster's blocks (at most 64), the
 // same in every thread: each warp's go to every block.  The slots of two rows
 // in turn: a warp that is ahead stores a row's sums while another still reads
-// the last row's.
+// the last row's.  Before the kernel's first row is joined, the blocks wait for
+// one another's cluster_arrive at the kernel's start: another block's shared
+// memory may be written only once that block runs.
 struct Slots {
   Sums of[2][64];
 };
-template <bool ENT> __device__ __forceinline__ Sums row_join(Sums mine, Slots &slots, unsigned part, unsigned parts, unsigned turn) {
+template <bool ENT> __device__ __forceinline__ Sums row_join(Sums mine, Slots &slots, unsigned part, unsigned parts, unsigned turn,
+                                                              bool first) {
   const unsigned lane = threadIdx.x & 31, warps = blockDim.x >> 5, n = parts * warps;
   Sums *all = slots.of[turn];
   mine = warp_join<ENT>(mine);
@@ -270,6 +273,7 @@ template <bool ENT> __device__ __forceinline__ Sums row_join(Sums mine, Slots &s
     if (lane == 0) all[threadIdx.x >> 5] = mine;
     __syncthreads();
   } else {
+    if (first) cluster_wait();
     if (lane < parts) {
       Sums *to = all + part * warps + (threadIdx.x >> 5);
       store_at(&to->m, lane, mine.m);
@@ -856,6 +860,7 @@ template <class T, bool ENT, int EXTRA> __global__ void __launch_bounds__(256, E
   const unsigned t = threadIdx.x, threads = blockDim.x, part = cluster_part(), parts = cluster_parts();
   const size_t first = blockIdx.x / parts, step = gridDim.x / parts;
   unsigned turn = 0;
+  if (parts > 1) cluster_arrive();  // waited for in the first row's join (every cluster has a row)
   for (size_t r = first; r < a.rows; r += step, turn ^= 1) {
     const S *row = static_cast<const S *>(a.logits) + r * a.stride;
     const Cut<T> c(row, a.vocab, part, parts);
@@ -873,7 +878,7 @@ template <class T, bool ENT, int EXTRA> __global__ void __launch_bounds__(256, E
           if (run.take(bits)) met = Met{c.body + i * V, unsigned(sizeof(bits) / sizeof(bits[0]))};
         });
     const Sums sums = run.sums();
-    const Sums all = row_join<ENT>(sums, joint, part, parts, turn);
+    const Sums all = row_join<ENT>(sums, joint, part, parts, turn, r == first);
     const Told o = told_by<ENT>(all);
     if (part == 0 && t == 0) write_told<ENT>(a, r, o, token, at_token);
     if constexpr (EXTRA == TOP) {
@@ -923,7 +928,7 @@ template <class T, bool ENT> __global__ void __launch_bounds__(256, 3) token_los
     if (t < c.head) run.take_one(T::load(row[t]));
     for (unsigned g = 0; g < groups; ++g) ring.each(g, c, [&](unsigned, const auto &bits) { run.take(bits); });
     if (t < c.tail) run.take_one(T::load(row[c.after + t]));
-    const Told o = told_by<ENT>(row_join<ENT>(run.sums(), joint, 0, 1, turn));
+    const Told o = told_by<ENT>(row_join<ENT>(run.sums(), joint, 0, 1, turn, false));
     if (t == 0) write_told<ENT>(a, r, o, token, at_token);
     const Slope s = slope_of(a, r, o.st, o.entropy);
     S *to = static_cast<S *>(a.grad_logits) + r * a.grad_stride;
@@ -967,6 +972,7 @@ template <class T, bool ENT> __global__ void __launch_bounds__(256, 4) token_los
   const unsigned t = threadIdx.x, threads = blockDim.x, part = cluster_part(), parts = cluster_parts();
   const size_t first = blockIdx.x / parts, step = gridDim.x / parts;
   unsigned turn = 0;
+  if (parts > 1) cluster_arrive();  // waited for in the first row's join (every cluster has a row)
   for (size_t r = first; r < a.rows; r += step, turn ^= 1) {
     const S *row = static_cast<const S *>(a.logits) + r * a.stride;
     const Cut<T> c(row, a.vocab, part, parts);
@@ -976,7 +982,7 @@ template <class T, bool ENT> __global__ void __launch_bounds__(256, 4) token_los
     walk<T>(
         row, c, t, threads, from_row<T>(row, c), [&](unsigned, S e) { run.take_one(T::load(e)); },
         [&](unsigned, const auto &bits) { run.take(bits); });
-    const Told o = told_by<ENT>(row_join<ENT>(run.sums(), joint, part, parts, turn));
+    const Told o = told_by<ENT>(row_join<ENT>(run.sums(), joint, part, parts, turn, r == first));
     if (part == 0 && t == 0) write_told<ENT>(a, r, o, token, at_token);
     write_slope<T, ENT>(row, static_cast<S *>(a.grad_logits) + r * a.grad_stride, c, slope_of(a, r, o.st, o.entropy), t, threads);
   }

@@ -159,10 +159,14 @@ __device__ __forceinline__ unsigned cluster_parts() {
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(v));
   return v;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
-// Store to the same variable of block `part`.
+// Store to the same variable of block `part`, which has to have started: a
+// kernel's first such store comes after a barrier of the cluster.
 template <class V> __device__ __forceinline__ void store_at(V *own, unsigned part, V v) {
   uint32_t to;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(uint32_t(__cvta_generic_to_shared(own))), "r"(part));
