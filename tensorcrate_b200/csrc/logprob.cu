@@ -731,7 +731,8 @@ template <class T, bool ENT, int EXTRA, int U> __global__ void __launch_bounds__
     // after them from lane 8 on
     const unsigned single = lane < c.head ? lane : lane >= 8 && lane - 8 < c.tail ? c.after + lane - 8 : ~0u;
     const float extra = single != ~0u ? T::load(row[single]) : -INFINITY;
-    const float in_runs = largest(bits), m = fmaxf(in_runs, extra);
+    // a lane of nothing but NaNs has no largest: -inf, as one without elements
+    const float in_runs = fmaxf(largest(bits), -INFINITY), m = fmaxf(in_runs, extra);
     float all_m = m;
 #pragma unroll
     for (int o = 16; o; o >>= 1) all_m = fmaxf(all_m, __shfl_xor_sync(0xffffffffu, all_m, o));

@@ -552,3 +552,26 @@ def test_on_a_stream_of_its_own(device):
     for a, b in zip(all_of(None), all_of(on)):
         assert np.array_equal(a, b)
     N.call("tc_ctx_destroy", ctx)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [9, 169, 337, 1001, 1003, 5003])
+def test_top_tokens_among_nans(device, vocab, dtype):
+    """NaNs rank last wherever they are: in all of a thread's 16-byte runs, in
+    the single elements before and after them, in all of the row."""
+    rng = np.random.default_rng(vocab)
+    x = np.full((8, vocab), np.nan)
+    x[1, -1], x[2, 0], x[3, vocab // 2] = 1.5, -2.0, 0.5
+    x[4, -1], x[4, -2] = -np.inf, -3.0
+    x[5] = np.where(rng.random(vocab) < 0.9, np.nan, rng.standard_normal(vocab))
+    x[6, -5:] = [2.0, 1.0, 2.0, 3.0, -np.inf]
+    x[7, :5] = [2.0, 1.0, 2.0, 3.0, -np.inf]
+    x = as_type(x, dtype)
+    for pad, offset in ((0, 0), (0, 1), (3, 5)):
+        X = matrix(x, dtype, pad, offset)
+        for top in (1, 5, 32):
+            top = min(top, vocab)
+            got = nn.token_logprobs(X, top=top)
+            want = np.argsort(-x, axis=1, kind="stable")[:, :top]  # NaNs sort last
+            assert np.array_equal(got.top_tokens.to_numpy(), want)
+            assert np.isnan(got.top_logprobs.to_f32()).all()
