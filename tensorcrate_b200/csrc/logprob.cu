@@ -100,10 +100,11 @@ template <class T, int U> __device__ __forceinline__ float largest(const Bits<T>
 
 // From here on a logit's weight is e = 2^a, a = x log2(e) - mark: one fused
 // operation.  The mark is m log2(e) rounded, which shifts every a of a row by
-// the same amount, known exactly, and is undone in what is taken from the
-// sums.  That holds for |m| up to TAME, where the shift is below 2^-13; past
-// it (a row masked by the type's lowest value, say) a = (x - m) log2(e), the
-// difference first.
+// the same amount, known exactly, and is undone where sums are restated for
+// another maximum and in what is taken from them.  That holds for |m| up to
+// TAME, where the shift is below 2^-13; past it (a row masked by the type's
+// lowest value, say) a = (x - m) log2(e), the difference first.  Weights below
+// 2^-126 are zero.
 constexpr float TAME = 1024.0f, LN2 = 0.6931471805599453f;
 __device__ __forceinline__ bool tame(float m) { return fabsf(m) <= TAME; }
 
@@ -146,7 +147,12 @@ template <class T, bool ENT> struct Running {
     const Running old = *this;
     begin(to);
     if (old.ref == -INFINITY) return;
-    const float up = old.wild || wild ? fminf((to - old.ref) * LOG2E, 1e20f) : mark - old.mark, f = exp2_of(-up);
+    float up = mark - old.mark;
+    if (old.wild || wild) {  // from or to a maximum itself, of which a mark is short by its rounding
+      const float rest = (old.wild ? 0.0f : fmaf(old.ref, LOG2E, -old.mark)) - (wild ? 0.0f : fmaf(to, LOG2E, -mark));
+      up = fminf((to - old.ref) * LOG2E + rest, 1e20f);
+    }
+    const float f = exp2_of(-up);
     if (ENT) t = mul2(pair(f, f), fma2(pair(-up, -up), s, t));
     s = mul2(pair(f, f), s);
   }

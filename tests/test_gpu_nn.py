@@ -575,3 +575,35 @@ def test_top_tokens_among_nans(device, vocab, dtype):
             want = np.argsort(-x, axis=1, kind="stable")[:, :top]  # NaNs sort last
             assert np.array_equal(got.top_tokens.to_numpy(), want)
             assert np.isnan(got.top_logprobs.to_f32()).all()
+
+
+@pytest.mark.parametrize("side", [1.0, -1.0])
+def test_a_maximum_that_passes_1024(device, side):
+    """Rows whose running maximum passes |x| = 1024 after many elements just
+    short of it: the weights are relative to a rounded multiple of the
+    maximum on one side and to the maximum itself on the other.  `to` is where
+    that rounding is largest.  Tolerance: as for all rows."""
+    vocab = 5003
+    near = np.float32(-1024.5 if side < 0 else 1023.0) + np.arange(64, dtype=np.float32) * np.float32(2.0 ** -13)
+    log2e = np.float32(1.4426950408889634)
+
+    def left(v):  # what rounding v * log2(e) to f32 leaves out
+        return np.abs(v.astype(np.float64) * np.float64(log2e) - (v * log2e).astype(np.float64))
+
+    at = near[np.argmax(left(near))]
+    later = np.float32(-1023.9) + np.arange(64, dtype=np.float32) * np.float32(2.0 ** -13)
+    to = later[np.argmax(left(later))] if side < 0 else at + np.float32(8.5)
+    four = np.full((4, vocab), at)
+    for r, first in enumerate((2200, 3000, 4000, 4900)):
+        four[r, first:] = to
+    four, token = as_type(four, "f32"), np.array([0, 4950, 1, 2], np.uint32)
+    lp, ent, m, ls = (np.tile(v, 300) for v in tokens64(four, token)[:4])
+    # so many rows that none is shared by blocks: each thread meets both values
+    X, tok = tensor(np.tile(four, (300, 1))), CudaStorage.store(np.tile(token, 300), "u32")
+    u = tensor(np.ones(1200))
+    for got in (nn.token_logprobs(X, tok), nn.token_loss(X, tok, u)[0]):
+        st = got.statistics.to_f32().astype(np.float64)
+        assert np.array_equal(st[:, 0], m)
+        within(st[:, 1], ls, 2.0 ** -18 + 2 * e * ls)
+        within(got.logprobs.to_f32(), lp, 2.0 ** -18 + 4 * e * (np.abs(lp) + 2 * ls))
+        within(got.entropy.to_f32(), ent, 2.0 ** -17 * (1 + ent + ls))
