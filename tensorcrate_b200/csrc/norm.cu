@@ -305,15 +305,16 @@ template <class T, int E, int K> struct Held {
     if constexpr (T::code == TC_F32) return pair(__uint_as_float(raw[2 * i]), __uint_as_float(raw[2 * i + 1]));
     else return widen2<T>(raw[i]);
   }
-  // The elements of `row` (in shared memory) at the columns of thread t;
-  // zeros past the row's end.
-  __device__ __forceinline__ void load(const typename T::S *row, unsigned t, unsigned threads, unsigned cols) {
+  // The elements of `row` (in shared memory) at the columns of thread t; past
+  // the row's end zeros, or (LAST) the row's last elements.
+  template <bool LAST> __device__ __forceinline__ void load(const typename T::S *row, unsigned t, unsigned threads, unsigned cols) {
     using S = typename T::S;
     if constexpr (E == 1) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const unsigned lo = t + 2 * i * threads, hi = lo + threads;
-        const S a = lo < cols ? row[lo] : S(0), b = hi < cols ? row[hi] : S(0);
+        const S a = LAST ? row[min(lo, cols - 1)] : lo < cols ? row[lo] : S(0);
+        const S b = LAST ? row[min(hi, cols - 1)] : hi < cols ? row[hi] : S(0);
         if constexpr (T::code == TC_F32) {
           raw[2 * i] = __float_as_uint(a);
           raw[2 * i + 1] = __float_as_uint(b);
@@ -325,7 +326,8 @@ template <class T, int E, int K> struct Held {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const unsigned c = (t + k * threads) * E;
-        const uint4 v = c < cols ? *reinterpret_cast<const uint4 *>(row + c) : make_uint4(0, 0, 0, 0);
+        const uint4 v = LAST || c < cols ? *reinterpret_cast<const uint4 *>(row + (LAST ? min(c, cols - E) : c))
+                                         : make_uint4(0, 0, 0, 0);
         raw[4 * k] = v.x;
         raw[4 * k + 1] = v.y;
         raw[4 * k + 2] = v.z;
@@ -433,10 +435,13 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       st[r] = next[r];
+      // A row past the last has no data: its gradient is zero, and its x the
+      // turn's first row's.  An element past the row's end has a zero gradient
+      // too, and the x of a real one: an h that is infinite for no other reason
+      // than that (0 - mean) rstd is would make the zeros' products NaN.
       const bool real = R == 1 || row + r < a.rows;
-      // a row past the last has no data: no columns of it are read
-      xr[r].load(held_at(2 * r, x_here + r * x_step), t, threads, real ? cols : 0);
-      gr[r].load(held_at(2 * r + 1, g_here + r * g_step), t, threads, real ? cols : 0);
+      xr[r].template load<true>(held_at(real ? 2 * r : 0, x_here + r * x_step), t, threads, cols);
+      gr[r].template load<false>(held_at(2 * r + 1, g_here + r * g_step), t, threads, real ? cols : 0);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -471,8 +476,7 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
     }
     row += every * R;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (row + r < a.rows) next[r] = a.statistics[row + r];
+    for (int r = 0; r < R; ++r) next[r] = row + r < a.rows ? a.statistics[row + r] : make_float2(0.0f, 0.0f);
     copy_wait<AHEAD - 2>();  // this thread's part of the next turn
     sync();
     // every thread is past the last turn, whose stage comes before this one
@@ -489,8 +493,8 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
         const float c1 = __shfl_sync(0xffffffffu, v, 16 * r) * st[r].y, c2 = __shfl_sync(0xffffffffu, v, 16 * r + 8) * st[r].y;
         if (R > 1 && row - every * R + r >= a.rows) break;
         const F2 mean = pair(-st[r].x, -st[r].x), rstd = pair(st[r].y, st[r].y), k1 = pair(c1, c1), k2 = pair(c2, c2);
-        xr[r].load(held_at(2 * r, x_here + r * x_step), t, threads, cols);
-        gr[r].load(held_at(2 * r + 1, g_here + r * g_step), t, threads, cols);
+        xr[r].template load<false>(held_at(2 * r, x_here + r * x_step), t, threads, cols);
+        gr[r].template load<false>(held_at(2 * r + 1, g_here + r * g_step), t, threads, cols);
 #pragma unroll
         for (int i = 0; i < N; i += STEP) {
           F2 out[STEP];

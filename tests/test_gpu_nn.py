@@ -607,3 +607,23 @@ def test_a_maximum_that_passes_1024(device, side):
         within(st[:, 1], ls, 2.0 ** -18 + 2 * e * ls)
         within(got.logprobs.to_f32(), lp, 2.0 ** -18 + 4 * e * (np.abs(lp) + 2 * ls))
         within(got.entropy.to_f32(), ent, 2.0 ** -17 * (1 + ent + ls))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(2, 64), (3, 256), (2, 33), (3, 16384)])
+def test_layer_norm_gradients_where_the_mean_is_near_the_largest_value(device, rows, cols, dtype):
+    """Rows of one value near the type's largest: their deviations are zero, so
+    grad_x = rstd (g w - mean(g w)), grad_weight is zero and all is finite.
+    What a thread holds beside the row's columns, or of a row past the last,
+    must not enter: (0 - mean) rstd is infinite there."""
+    value, eps = float(2.0 ** 121), 1e-5  # times rstd = 316: past 2^128
+    x, g = np.full((rows, cols), value), as_type(normal((rows, cols), 2), dtype)
+    st = tensor(np.tile([value, eps ** -0.5], (rows, 1)))
+    rstd = float(np.float32(eps ** -0.5))
+    dx, dw, db = nn.layer_norm_backward(tensor(g, dtype), tensor(x, dtype), st)
+    want = rstd * (g - g.mean(1, keepdims=True))
+    # as in test_layer_norm_and_its_gradients, with h = 0
+    within(dx.to_f32(), want, U[dtype] * np.abs(want) + 48 * e * rstd * (np.abs(g) + np.abs(g).mean(1, keepdims=True)))
+    assert not dw.to_f32().any()
+    want = g.sum(0)
+    within(db.to_f32(), want, U[dtype] * np.abs(want) + 128 * e * np.abs(g).sum(0))
