@@ -130,12 +130,16 @@ int tc_ctx_destroy(tc_ctx *ctx);
  * before the call may still use it): a later tc_malloc_async on the same
  * stream may take it at once, a request on another stream only with that
  * stream made to wait for the freeing stream's work, and tc_malloc only once
- * that work has completed.  This is how a storage dropped while its
- * kernels are queued (Drop of `CudaStorage`) goes back to the pool. */
+ * that work has completed.  tc_free_shared returns it in `stream`'s order and
+ * in that of the stream tc_malloc_async was given for it, which has to exist
+ * still, or to be that of a context that tc_ctx_destroy ended.  This is how a
+ * storage dropped while its kernels are queued (Drop of `CudaStorage`) goes
+ * back to the pool. */
 int tc_malloc(void **out_dev, size_t bytes);
 int tc_malloc_async(void **out_dev, size_t bytes, void *stream);
 int tc_free(void *dev);
 int tc_free_async(void *dev, void *stream);
+int tc_free_shared(void *dev, void *stream);
 /* Release every cached block back to CUDA. */
 int tc_pool_trim(void);
 /* Counters since the library loaded: cudaMalloc calls the library made

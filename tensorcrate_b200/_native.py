@@ -109,6 +109,7 @@ SIGNATURES = {
     "tc_malloc_async": [C.POINTER(_p), _sz, _p],
     "tc_free": [_p],
     "tc_free_async": [_p, _p],
+    "tc_free_shared": [_p, _p],
     "tc_alloc_counts": [C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)],
     "tc_pool_trim": [],
     "tc_host_alloc": [C.POINTER(_p), _sz],

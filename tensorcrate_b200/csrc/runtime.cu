@@ -175,16 +175,27 @@ void release_stream_blocks(int dev, cudaStream_t stream) {
 // only in that stream's order: at once to a request on the same stream,
 // after the event has completed to tc_malloc, and to tc_malloc_async on
 // another stream with that stream made to wait for the event.
+// tc_free_shared does so for two streams, the given one and the one that the
+// block was allocated on.
 // ---------------------------------------------------------------------------
+struct Use {
+  uintptr_t stream;  // a stream that the block was freed on
+  cudaEvent_t done;  // recorded there; null: no queued work of it uses the block
+};
 struct FreeBlock {
   void *ptr;
-  uintptr_t stream;  // the stream it was freed on (tc_free_async)
-  cudaEvent_t done;  // recorded there; null: no queued work uses the block
+  Use uses[2];
+};
+struct LiveBlock {
+  int dev;
+  size_t cls;
+  bool has_home;   // allocated on a stream that was not since destroyed by tc_ctx_destroy
+  uintptr_t home;  // that stream
 };
 struct Pool {
   std::mutex mu;
   std::map<std::pair<int, size_t>, std::vector<FreeBlock>> free_blocks;
-  std::unordered_map<void *, std::pair<int, size_t>> live;
+  std::unordered_map<void *, LiveBlock> live;
   std::vector<cudaEvent_t> spare_events;
 };
 Pool &pool() {
@@ -211,31 +222,32 @@ bool take_cached(Pool &p, int dev, size_t cls, bool has_stream, cudaStream_t str
   if (it == p.free_blocks.end() || it->second.empty()) return false;
   auto &v = it->second;
   const uintptr_t key = reinterpret_cast<uintptr_t>(stream);
+  auto ordered = [&](const Use &u) { return !u.done || (has_stream && u.stream == key); };
+  auto finished = [&](const Use &u) {
+    if (ordered(u) || cudaEventQuery(u.done) == cudaSuccess) return true;
+    cudaGetLastError();  // cudaErrorNotReady is not a failure
+    return false;
+  };
   int pick = -1;
-  bool wait = false;
   for (int pass = 0; pass < 3 && pick < 0; ++pass) {
     for (int i = int(v.size()) - 1; i >= 0 && pick < 0; --i) {
       const FreeBlock &f = v[size_t(i)];
-      if (pass == 0) {
-        if (!f.done || (has_stream && f.stream == key)) pick = i;
-      } else if (pass == 1) {
-        if (cudaEventQuery(f.done) == cudaSuccess) pick = i;
-        else cudaGetLastError();  // cudaErrorNotReady is not a failure
-      } else if (has_stream) {
+      if (pass == 0 ? ordered(f.uses[0]) && ordered(f.uses[1])
+                    : pass == 1 ? finished(f.uses[0]) && finished(f.uses[1]) : has_stream)
         pick = i;
-        wait = true;
-      }
     }
   }
   if (pick < 0) return false;
   FreeBlock f = v[size_t(pick)];
   v.erase(v.begin() + pick);
-  if (wait && cudaStreamWaitEvent(stream, f.done, 0) != cudaSuccess) {
-    cudaGetLastError();
-    cudaEventSynchronize(f.done);
+  for (const Use &u : f.uses) {
+    if (!finished(u) && cudaStreamWaitEvent(stream, u.done, 0) != cudaSuccess) {
+      cudaGetLastError();
+      cudaEventSynchronize(u.done);
+    }
+    if (u.done) p.spare_events.push_back(u.done);
   }
-  if (f.done) p.spare_events.push_back(f.done);
-  p.live[f.ptr] = {dev, cls};
+  p.live[f.ptr] = {dev, cls, has_stream, key};
   *out = f.ptr;
   return true;
 }
@@ -263,36 +275,51 @@ int pool_malloc(void **out, size_t bytes, bool has_stream, cudaStream_t stream) 
   }
   if (err != cudaSuccess) return check_cuda(err, "cudaMalloc");
   std::lock_guard<std::mutex> g(p.mu);
-  p.live[ptr] = {dev, cls};
+  p.live[ptr] = {dev, cls, has_stream, reinterpret_cast<uintptr_t>(stream)};
   *out = ptr;
   return TC_OK;
 }
 
-int pool_free(void *dev_ptr, bool has_stream, cudaStream_t stream) {
+// An event recorded on `stream` (with the pool's lock held).
+int record_use(Pool &p, uintptr_t stream, Use *out) {
+  cudaEvent_t e = nullptr;
+  if (!p.spare_events.empty()) {
+    e = p.spare_events.back();
+    p.spare_events.pop_back();
+  } else if (int st = check_cuda(cudaEventCreateWithFlags(&e, cudaEventDisableTiming), "cudaEventCreate")) {
+    return st;
+  }
+  if (int st = check_cuda(cudaEventRecord(e, reinterpret_cast<cudaStream_t>(stream)), "cudaEventRecord")) {
+    p.spare_events.push_back(e);
+    return st;
+  }
+  *out = {stream, e};
+  return TC_OK;
+}
+
+int pool_free(void *dev_ptr, bool has_stream, cudaStream_t stream, bool with_home) {
   if (!dev_ptr) return TC_OK;
   Pool &p = pool();
   std::lock_guard<std::mutex> g(p.mu);
   auto it = p.live.find(dev_ptr);
   if (it == p.live.end()) return fail(TC_EINVAL, "tc_free: %p was not allocated by tc_malloc", dev_ptr);
-  FreeBlock f{dev_ptr, reinterpret_cast<uintptr_t>(stream), nullptr};
-  if (has_stream) {
-    if (!p.spare_events.empty()) {
-      f.done = p.spare_events.back();
-      p.spare_events.pop_back();
-    } else if (int st = check_cuda(cudaEventCreateWithFlags(&f.done, cudaEventDisableTiming), "cudaEventCreate")) {
+  const LiveBlock &b = it->second;
+  FreeBlock f{dev_ptr, {}};
+  const uintptr_t key = reinterpret_cast<uintptr_t>(stream);
+  if (has_stream)
+    if (int st = record_use(p, key, &f.uses[0])) return st;
+  if (with_home && b.has_home && b.home != key)
+    if (int st = record_use(p, b.home, &f.uses[1])) {
+      if (f.uses[0].done) p.spare_events.push_back(f.uses[0].done);
       return st;
     }
-    if (int st = check_cuda(cudaEventRecord(f.done, stream), "cudaEventRecord")) {
-      p.spare_events.push_back(f.done);
-      return st;
-    }
-  }
-  p.free_blocks[it->second].push_back(f);
+  p.free_blocks[{b.dev, b.cls}].push_back(f);
   p.live.erase(it);
   return TC_OK;
 }
 
-// After `stream` is idle: its freed blocks need no more ordering.
+// After `stream` is idle, and about to be destroyed: the blocks freed on it
+// need no more ordering, and those allocated on it have no stream any more.
 void settle_stream_blocks(int dev, cudaStream_t stream) {
   Pool &p = pool();
   std::lock_guard<std::mutex> g(p.mu);
@@ -300,11 +327,14 @@ void settle_stream_blocks(int dev, cudaStream_t stream) {
   for (auto &kv : p.free_blocks) {
     if (kv.first.first != dev) continue;
     for (FreeBlock &f : kv.second)
-      if (f.done && f.stream == key) {
-        p.spare_events.push_back(f.done);
-        f.done = nullptr;
-      }
+      for (Use &u : f.uses)
+        if (u.done && u.stream == key) {
+          p.spare_events.push_back(u.done);
+          u.done = nullptr;
+        }
   }
+  for (auto &kv : p.live)
+    if (kv.second.dev == dev && kv.second.home == key) kv.second.has_home = false;
 }
 }  // namespace
 
@@ -347,8 +377,9 @@ int tc_sm_count(int *count) {
 
 int tc_malloc(void **out, size_t bytes) { return pool_malloc(out, bytes, false, nullptr); }
 int tc_malloc_async(void **out, size_t bytes, void *stream) { return pool_malloc(out, bytes, true, as_stream(stream)); }
-int tc_free(void *dev_ptr) { return pool_free(dev_ptr, false, nullptr); }
-int tc_free_async(void *dev_ptr, void *stream) { return pool_free(dev_ptr, true, as_stream(stream)); }
+int tc_free(void *dev_ptr) { return pool_free(dev_ptr, false, nullptr, false); }
+int tc_free_async(void *dev_ptr, void *stream) { return pool_free(dev_ptr, true, as_stream(stream), false); }
+int tc_free_shared(void *dev_ptr, void *stream) { return pool_free(dev_ptr, true, as_stream(stream), true); }
 
 int tc_pool_trim(void) {
   Pool &p = pool();
@@ -363,10 +394,11 @@ int tc_pool_trim(void) {
   cudaGetDevice(&cur);
   for (auto &b : blocks) {
     cudaSetDevice(b.first);
-    if (b.second.done) {
-      cudaEventSynchronize(b.second.done);
-      cudaEventDestroy(b.second.done);
-    }
+    for (const Use &u : b.second.uses)
+      if (u.done) {
+        cudaEventSynchronize(u.done);
+        cudaEventDestroy(u.done);
+      }
     cudaFree(b.second.ptr);
   }
   cudaSetDevice(cur);

@@ -76,20 +76,24 @@ def _stream(stream) -> C.c_void_p:
 # ---------------------------------------------------------------------------
 class CudaStorage:
     """A flat run of `len` elements of `dtype` in device memory.  Its block
-    comes from the library's pool in the default stream's order and goes
-    back in that order when the storage is dropped (tc_free_async), so a
-    storage dropped while kernels that use it are queued is not handed out
-    before they ran."""
+    comes from the library's pool in the order of `stream` (the default
+    stream's unless given; the results that a call on a stream makes are made on
+    that one), and goes back in that stream's and in the default stream's order
+    when the storage is dropped (tc_free_shared).  So it is not written before
+    its last use, and a storage dropped while kernels of either stream that use
+    it are queued is not handed out before they ran.  A stream has to exist as
+    long as the storages made on it; one of tc_ctx_create's may go before
+    them."""
 
     __slots__ = ("ptr", "len", "dtype", "_owned", "__weakref__")
 
-    def __init__(self, dtype: str, length: int, ptr: int | None = None):
+    def __init__(self, dtype: str, length: int, ptr: int | None = None, stream=None):
         if dtype not in ELEM:
             raise ValueError(f"unknown element type {dtype!r}")
         self.dtype, self.len = dtype, int(length)
         if ptr is None:
             out = C.c_void_p()
-            N.call("tc_malloc_async", C.byref(out), max(1, self.len * ELEM[dtype][1]), None)
+            N.call("tc_malloc_async", C.byref(out), max(1, self.len * ELEM[dtype][1]), _stream(stream))
             self.ptr, self._owned = out.value, True
         else:
             self.ptr, self._owned = int(ptr), False
@@ -106,7 +110,7 @@ class CudaStorage:
     def store(cls, values, dtype: str, stream=None) -> "CudaStorage":
         """Backend::store: upload `values` (already in `dtype`'s storage form)."""
         host = np.ascontiguousarray(values, dtype=ELEM[dtype][0]).reshape(-1)
-        s = cls(dtype, host.size)
+        s = cls(dtype, host.size, stream=stream)
         if host.size:
             N.call("tc_memcpy_h2d", s.ptr, host.ctypes.data, host.nbytes, _stream(stream))
             if stream is None:
@@ -132,7 +136,7 @@ class CudaStorage:
         return bits_to_f32(self.as_slice(), self.dtype)
 
     def duplicate(self, stream=None) -> "CudaStorage":
-        s = CudaStorage(self.dtype, self.len)
+        s = CudaStorage(self.dtype, self.len, stream=stream)
         if self.len:
             N.call("tc_memcpy_d2d", s.ptr, self.ptr, self.nbytes, _stream(stream))
         return s
@@ -140,7 +144,7 @@ class CudaStorage:
     def __del__(self):
         try:
             if self._owned and self.ptr and N._lib is not None:
-                N._lib.tc_free_async(self.ptr, None)
+                N._lib.tc_free_shared(self.ptr, None)
         except Exception:  # interpreter shutdown
             pass
 
@@ -393,7 +397,7 @@ def elementwise(a, b, kind: int, op: int, stream=None) -> Tensor:
     if a.dtype != b.dtype:
         raise ValueError("elementwise: element types differ")
     if a.shape == b.shape and a.is_whole() and b.is_whole():
-        out = CudaStorage(a.dtype, a.numel())
+        out = CudaStorage(a.dtype, a.numel(), stream=stream)
         fn = {N.PAIR_ARITHMETIC: "tc_elementwise", N.PAIR_COMPARE: "tc_compare"}.get(kind)
         if fn is not None:
             N.call(fn, N.DTYPES[a.dtype], op, a.storage.ptr, b.storage.ptr, out.ptr, out.len, _stream(stream))
@@ -462,7 +466,7 @@ class Cuda:
     @staticmethod
     def strided_copy(storage: CudaStorage, shape, offset: int, strides, stream=None) -> CudaStorage:
         n = int(np.prod(shape, dtype=np.int64)) if shape else 1
-        out = CudaStorage(storage.dtype, n)
+        out = CudaStorage(storage.dtype, n, stream=stream)
         N.call("tc_strided_copy", storage.elem_bytes, len(shape), N.sizes(shape), storage.ptr, storage.len,
                offset, N.sizes(strides), out.ptr, _stream(stream))
         return out
@@ -480,7 +484,7 @@ class Cuda:
     @staticmethod
     def assemble(dtype: str, length: int, regions, stream=None) -> CudaStorage:
         """regions: (source, shape, from_offset, from_strides, to_offset, to_strides)."""
-        out = CudaStorage(dtype, length)
+        out = CudaStorage(dtype, length, stream=stream)
         arr = (N.Region * max(1, len(regions)))(*[Cuda._region(r) for r in regions])
         N.call("tc_assemble", ELEM[dtype][1], out.ptr, length, arr, len(regions), _stream(stream))
         return out
@@ -495,13 +499,13 @@ class Cuda:
     def vector_elementwise(a: CudaStorage, b: CudaStorage, op: int, stream=None) -> CudaStorage:
         if a.len != b.len:
             raise ValueError(f"elementwise: lengths {a.len} and {b.len} differ")
-        out = CudaStorage(a.dtype, a.len)
+        out = CudaStorage(a.dtype, a.len, stream=stream)
         N.call("tc_elementwise", N.DTYPES[a.dtype], op, a.ptr, b.ptr, out.ptr, a.len, _stream(stream))
         return out
 
     @staticmethod
     def vector_broadcast(a: CudaStorage, scalar: float, op: int, scalar_left: bool, stream=None) -> CudaStorage:
-        out = CudaStorage(a.dtype, a.len)
+        out = CudaStorage(a.dtype, a.len, stream=stream)
         N.call("tc_broadcast_scalar", N.DTYPES[a.dtype], op, a.ptr, float(scalar), int(scalar_left), out.ptr,
                a.len, _stream(stream))
         return out
@@ -510,51 +514,51 @@ class Cuda:
     def vector_compare(a: CudaStorage, b: CudaStorage, op: int, stream=None) -> CudaStorage:
         if a.len != b.len:
             raise ValueError(f"compare: lengths {a.len} and {b.len} differ")
-        out = CudaStorage(a.dtype, a.len)
+        out = CudaStorage(a.dtype, a.len, stream=stream)
         N.call("tc_compare", N.DTYPES[a.dtype], op, a.ptr, b.ptr, out.ptr, a.len, _stream(stream))
         return out
 
     @staticmethod
     def vector_compare_scalar(a: CudaStorage, scalar: float, op: int, scalar_left: bool, stream=None):
-        out = CudaStorage(a.dtype, a.len)
+        out = CudaStorage(a.dtype, a.len, stream=stream)
         N.call("tc_compare_scalar", N.DTYPES[a.dtype], op, a.ptr, float(scalar), int(scalar_left), out.ptr,
                a.len, _stream(stream))
         return out
 
     @staticmethod
     def vector_clamp(a: CudaStorage, low: float, high: float, stream=None) -> CudaStorage:
-        out = CudaStorage(a.dtype, a.len)
+        out = CudaStorage(a.dtype, a.len, stream=stream)
         N.call("tc_clamp", N.DTYPES[a.dtype], a.ptr, float(low), float(high), out.ptr, a.len, _stream(stream))
         return out
 
     @staticmethod
     def vector_reduce(a: CudaStorage, op: int, stream=None) -> CudaStorage:
-        out = CudaStorage(a.dtype, 1)
+        out = CudaStorage(a.dtype, 1, stream=stream)
         N.call("tc_vector_reduce", N.DTYPES[a.dtype], op, a.ptr, a.len, out.ptr, _stream(stream))
         return out
 
     @staticmethod
     def dot(a: CudaStorage, b: CudaStorage, stream=None) -> CudaStorage:
-        out = CudaStorage(a.dtype, 1)
+        out = CudaStorage(a.dtype, 1, stream=stream)
         N.call("tc_dot", N.DTYPES[a.dtype], a.ptr, b.ptr, a.len, out.ptr, _stream(stream))
         return out
 
     @staticmethod
     def vector_prefix_sum(a: CudaStorage, stream=None) -> CudaStorage:
-        out = CudaStorage(a.dtype, a.len)
+        out = CudaStorage(a.dtype, a.len, stream=stream)
         N.call("tc_prefix_sum", N.DTYPES[a.dtype], a.ptr, out.ptr, a.len, _stream(stream))
         return out
 
     @staticmethod
     def vector_sort(a: CudaStorage, order: int, stream=None) -> CudaStorage:
-        out = CudaStorage(a.dtype, a.len)
+        out = CudaStorage(a.dtype, a.len, stream=stream)
         N.call("tc_sort", N.DTYPES[a.dtype], order, a.ptr, out.ptr, a.len, _stream(stream))
         return out
 
     @staticmethod
     def vector_unary(a: CudaStorage, f: int, stream=None) -> CudaStorage:
         """vector_unary / matrix_unary: f an Analytic."""
-        out = CudaStorage(a.dtype, a.len)
+        out = CudaStorage(a.dtype, a.len, stream=stream)
         N.call("tc_unary", N.DTYPES[a.dtype], f, a.ptr, out.ptr, a.len, _stream(stream))
         return out
 
@@ -563,7 +567,7 @@ class Cuda:
                           stream=None) -> tuple[CudaStorage, CudaStorage]:
         if value.len != tangent.len:
             raise ValueError("unary_dual: value and tangent lengths differ")
-        out_v, out_t = CudaStorage(value.dtype, value.len), CudaStorage(value.dtype, value.len)
+        out_v, out_t = (CudaStorage(value.dtype, value.len, stream=stream) for _ in range(2))
         N.call("tc_unary_dual", N.DTYPES[value.dtype], f, value.ptr, tangent.ptr, out_v.ptr, out_t.ptr, value.len,
                _stream(stream))
         return out_v, out_t
@@ -572,13 +576,13 @@ class Cuda:
     def vector_power(a: CudaStorage, b: CudaStorage, stream=None) -> CudaStorage:
         if a.len != b.len:
             raise ValueError(f"pow: lengths {a.len} and {b.len} differ")
-        out = CudaStorage(a.dtype, a.len)
+        out = CudaStorage(a.dtype, a.len, stream=stream)
         N.call("tc_power", N.DTYPES[a.dtype], a.ptr, b.ptr, out.ptr, a.len, _stream(stream))
         return out
 
     @staticmethod
     def vector_power_scalar(a: CudaStorage, scalar: float, scalar_left: bool, stream=None) -> CudaStorage:
-        out = CudaStorage(a.dtype, a.len)
+        out = CudaStorage(a.dtype, a.len, stream=stream)
         N.call("tc_power_scalar", N.DTYPES[a.dtype], a.ptr, float(scalar), int(scalar_left), out.ptr, a.len,
                _stream(stream))
         return out
@@ -590,7 +594,7 @@ class Cuda:
         (r, c), (wr, wc) = shape, window_shape
         if wr > r or wc > c:
             raise ValueError(f"correlate: a {wr}x{wc} window does not fit in a {r}x{c} input")
-        out = CudaStorage(input.dtype, (r - wr + 1) * (c - wc + 1))
+        out = CudaStorage(input.dtype, (r - wr + 1) * (c - wc + 1), stream=stream)
         N.call("tc_correlate", N.DTYPES[input.dtype], r, c, wr, wc, int(flip), input.ptr, window.ptr, out.ptr,
                _stream(stream))
         return out
@@ -604,7 +608,7 @@ class Cuda:
     def correlate_input_gradient(adjoint: CudaStorage, adjoint_shape, window: CudaStorage, window_shape,
                                  forward_flip: bool, stream=None) -> CudaStorage:
         (ar, ac), (wr, wc) = adjoint_shape, window_shape
-        out = CudaStorage(adjoint.dtype, (ar + wr - 1) * (ac + wc - 1))
+        out = CudaStorage(adjoint.dtype, (ar + wr - 1) * (ac + wc - 1), stream=stream)
         N.call("tc_correlate_input_gradient", N.DTYPES[adjoint.dtype], ar, ac, wr, wc, int(forward_flip),
                adjoint.ptr, window.ptr, out.ptr, _stream(stream))
         return out
@@ -612,14 +616,14 @@ class Cuda:
     @staticmethod
     def pad(input: CudaStorage, shape, pad_rows: int, pad_cols: int, stream=None) -> CudaStorage:
         r, c = shape
-        out = CudaStorage(input.dtype, (r + 2 * pad_rows) * (c + 2 * pad_cols))
+        out = CudaStorage(input.dtype, (r + 2 * pad_rows) * (c + 2 * pad_cols), stream=stream)
         N.call("tc_pad", N.DTYPES[input.dtype], r, c, pad_rows, pad_cols, input.ptr, out.ptr, _stream(stream))
         return out
 
     @staticmethod
     def flip(input: CudaStorage, shape, stream=None) -> CudaStorage:
         r, c = shape
-        out = CudaStorage(input.dtype, r * c)
+        out = CudaStorage(input.dtype, r * c, stream=stream)
         N.call("tc_flip", N.DTYPES[input.dtype], r, c, input.ptr, out.ptr, _stream(stream))
         return out
 
@@ -627,7 +631,7 @@ class Cuda:
     @staticmethod
     def vector_moments(a: CudaStorage, stream=None) -> CudaStorage:
         """(mean, deviations) as a 2-element device vector."""
-        out = CudaStorage(a.dtype, 2)
+        out = CudaStorage(a.dtype, 2, stream=stream)
         N.call("tc_moments", N.DTYPES[a.dtype], a.ptr, a.len, out.ptr, _stream(stream))
         return out
 
@@ -635,13 +639,13 @@ class Cuda:
     def matrix_axis_moments(a: CudaStorage, shape, axis: int, stream=None) -> tuple[CudaStorage, CudaStorage]:
         r, c = shape
         extent = r if axis == N.ROWS else c
-        means, devs = CudaStorage(a.dtype, extent), CudaStorage(a.dtype, extent)
+        means, devs = CudaStorage(a.dtype, extent, stream=stream), CudaStorage(a.dtype, extent, stream=stream)
         N.call("tc_axis_moments", N.DTYPES[a.dtype], r, c, axis, a.ptr, means.ptr, devs.ptr, _stream(stream))
         return means, devs
 
     @staticmethod
     def vector_distribution(a: CudaStorage, family: int, statistic: int, parameters, stream=None) -> CudaStorage:
-        out = CudaStorage(a.dtype, a.len)
+        out = CudaStorage(a.dtype, a.len, stream=stream)
         N.call("tc_distribution", N.DTYPES[a.dtype], family, statistic, a.ptr, a.len, float(parameters[0]),
                float(parameters[1]), out.ptr, _stream(stream))
         return out
@@ -650,7 +654,7 @@ class Cuda:
     def matrix_axis_distribution(a: CudaStorage, shape, axis: int, family: int, statistic: int,
                                  first: CudaStorage, second: CudaStorage, stream=None) -> CudaStorage:
         r, c = shape
-        out = CudaStorage(a.dtype, r * c)
+        out = CudaStorage(a.dtype, r * c, stream=stream)
         N.call("tc_axis_distribution", N.DTYPES[a.dtype], r, c, axis, family, statistic, a.ptr, first.ptr,
                second.ptr, out.ptr, _stream(stream))
         return out
@@ -661,7 +665,7 @@ class Cuda:
                addend: CudaStorage | None = None, stream=None) -> CudaStorage:
         """matmul / matmul_add / matmul_transposed_add: `addend` is consumed as
         the accumulator (kernels.rs:958-985)."""
-        out = addend if addend is not None else CudaStorage(a.dtype, rows * cols)
+        out = addend if addend is not None else CudaStorage(a.dtype, rows * cols, stream=stream)
         N.call("tc_matmul", N.DTYPES[a.dtype], transposed, rows, inner, cols, a.ptr, b.ptr, out.ptr,
                int(addend is not None), _stream(stream))
         return out
@@ -669,14 +673,14 @@ class Cuda:
     @staticmethod
     def matvec(m: CudaStorage, v: CudaStorage, rows: int, cols: int, addend: CudaStorage | None = None,
                stream=None) -> CudaStorage:
-        out = addend if addend is not None else CudaStorage(m.dtype, rows)
+        out = addend if addend is not None else CudaStorage(m.dtype, rows, stream=stream)
         N.call("tc_matvec", N.DTYPES[m.dtype], rows, cols, m.ptr, v.ptr, out.ptr, int(addend is not None),
                _stream(stream))
         return out
 
     @staticmethod
     def vecmat(v: CudaStorage, m: CudaStorage, rows: int, cols: int, stream=None) -> CudaStorage:
-        out = CudaStorage(m.dtype, cols)
+        out = CudaStorage(m.dtype, cols, stream=stream)
         N.call("tc_vecmat", N.DTYPES[m.dtype], rows, cols, v.ptr, m.ptr, out.ptr, _stream(stream))
         return out
 
@@ -689,7 +693,7 @@ class Cuda:
     def strided_binary(a: TensorView, b: TensorView, kind: int, op: int, stream=None) -> CudaStorage:
         if list(a.shape) != list(b.shape):
             raise ValueError("strided binary: the operands' shapes differ")
-        out = CudaStorage(a.dtype, a.numel())
+        out = CudaStorage(a.dtype, a.numel(), stream=stream)
         N.call("tc_strided_binary", N.DTYPES[a.dtype], kind, op, a.rank, N.sizes(a.shape), a.storage.ptr,
                a.storage.len, a.offset, N.sizes(a.strides), b.storage.ptr, b.storage.len, b.offset,
                N.sizes(b.strides), out.ptr, _stream(stream))
@@ -699,7 +703,7 @@ class Cuda:
     def reduce_axes(view: TensorView, axes: Sequence[int], kind: int, op: int, divisor: int,
                     stream=None) -> CudaStorage:
         results = int(np.prod([e for a, e in enumerate(view.shape) if a not in axes], dtype=np.int64))
-        out = CudaStorage(view.dtype, results)
+        out = CudaStorage(view.dtype, results, stream=stream)
         N.call("tc_reduce_axes", N.DTYPES[view.dtype], view.rank, N.sizes(view.shape), view.storage.ptr,
                view.storage.len, view.offset, N.sizes(view.strides), len(axes), N.u32s(axes), kind, op,
                divisor, out.ptr, _stream(stream))
@@ -708,7 +712,7 @@ class Cuda:
     @staticmethod
     def arg_reduce(view: TensorView, axis: int, op: int, stream=None) -> CudaStorage:
         results = int(np.prod([e for a, e in enumerate(view.shape) if a != axis], dtype=np.int64))
-        out = CudaStorage("u32", results)
+        out = CudaStorage("u32", results, stream=stream)
         N.call("tc_arg_reduce", N.DTYPES[view.dtype], view.rank, N.sizes(view.shape), view.storage.ptr,
                view.storage.len, view.offset, N.sizes(view.strides), axis, op,
                C.cast(C.c_void_p(out.ptr), C.POINTER(C.c_uint32)), _stream(stream))

@@ -6,7 +6,10 @@ clipping of gradients by their global norm.
 Matrices are Tensors or TensorViews of any rank >= 1 whose last axis has its
 elements side by side; the leading axes are the rows and have to step as one
 axis (any contiguous tensor, a slice of one along its first or last axis).
-Results go to the `out` arguments where they are given, else to new tensors.
+Results go to the `out` arguments where they are given, else to new tensors,
+made in the order of the call's stream (CudaStorage says how they go back);
+an argument made on another stream is the caller's to order, and to keep until
+the call has run.
 Shapes that do not fit raise ValueError; the library's own refusals raise
 TcError.  Nothing waits for the device.
 """
@@ -96,11 +99,11 @@ def _vector(what: str, x, n: int, dtypes: Sequence[str]) -> int | None:
     return storage.ptr + offset * _BYTES[storage.dtype]
 
 
-def _like(x, shape, dtype: str) -> Tensor:
+def _new(shape, dtype: str, stream) -> Tensor:
     n = 1
     for e in shape:
         n *= e
-    return Tensor(CudaStorage(dtype, n), shape)
+    return Tensor(CudaStorage(dtype, n, stream=stream), shape)
 
 
 def _same_shape(what: str, x, y) -> None:
@@ -124,12 +127,12 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None, statistic
     if weight is not None and bias is not None and _dtype(bias) != kind:
         raise ValueError(f"layer_norm: weight is {kind}, bias {_dtype(bias)}")
     if out is None:
-        out = _like(x, x.shape, dtype)
+        out = _new(x.shape, dtype, stream)
     else:
         _same_shape("layer_norm", x, out)
     yptr, _, _, ystride = _matrix("layer_norm: out", out, dtype)
     if statistics is None:
-        statistics = _like(x, [rows, 2], "f32")
+        statistics = _new([rows, 2], "f32", stream)
     st = _vector("layer_norm: statistics", statistics, 2 * rows, ("f32",))
     _run("tc_layer_norm", stream, N.DTYPES[dtype], N.DTYPES[kind], rows, cols, ptr, stride, w, b, eps, yptr, ystride, st)
     return out, statistics
@@ -151,14 +154,14 @@ def layer_norm_backward(grad, x, statistics, weight=None, out=None, grad_weight=
     kind = _dtype(weight) or _dtype(grad_weight) or _dtype(grad_bias) or dtype
     st = _vector("layer_norm_backward: statistics", statistics, 2 * rows, ("f32",))
     if out is None:
-        out = _like(x, x.shape, dtype)
+        out = _new(x.shape, dtype, stream)
     else:
         _same_shape("layer_norm_backward", x, out)
     optr, _, _, ostride = _matrix("layer_norm_backward: out", out, dtype)
     if grad_weight is None:
-        grad_weight = _like(x, [cols], kind)
+        grad_weight = _new([cols], kind, stream)
     if grad_bias is None:
-        grad_bias = _like(x, [cols], kind)
+        grad_bias = _new([cols], kind, stream)
     gw = _vector("layer_norm_backward: grad_weight", grad_weight, cols, (kind,))
     gb = _vector("layer_norm_backward: grad_bias", grad_bias, cols, (kind,))
     _run("tc_layer_norm_backward", stream, N.DTYPES[dtype], N.DTYPES[kind], rows, cols, gptr, gstride, ptr, stride, st, w,
@@ -181,9 +184,9 @@ class TokenLogprobs:
     top_logprobs: object = None
 
 
-def _fresh(rows: int, tokens, entropy: bool, top: int) -> TokenLogprobs:
+def _fresh(rows: int, tokens, entropy: bool, top: int, stream) -> TokenLogprobs:
     def new(shape, dtype="f32"):
-        return _like(None, shape, dtype)
+        return _new(shape, dtype, stream)
 
     return TokenLogprobs(new([rows]) if tokens is not None else None, new([rows]) if entropy else None, new([rows, 2]),
                          new([rows, top], "u32") if top else None, new([rows, top]) if top else None)
@@ -205,7 +208,7 @@ def token_logprobs(logits, tokens=None, top: int = 0, entropy: bool = True, out:
     ptr, rows, vocab, stride = _matrix("token_logprobs: logits", logits)
     tok = _vector("token_logprobs: tokens", tokens, rows, ("u32",))
     if out is None:
-        out = _fresh(rows, tokens, entropy, top)
+        out = _fresh(rows, tokens, entropy, top, stream)
     elif (out.top_tokens is None) != (out.top_logprobs is None):
         raise ValueError("token_logprobs: top_tokens and top_logprobs go together")
     else:
@@ -231,7 +234,7 @@ def token_logprobs_backward(logits, tokens, statistics, grad_logprobs=None, entr
                                   ("grad_logprobs", grad_logprobs, "f32"), ("grad_entropy", grad_entropy, "f32"))]
     st = _vector("token_logprobs_backward: statistics", statistics, 2 * rows, ("f32",))
     if out is None:
-        out = _like(logits, logits.shape, dtype)
+        out = _new(logits.shape, dtype, stream)
     else:
         _same_shape("token_logprobs_backward", logits, out)
     optr, _, _, ostride = _matrix("token_logprobs_backward: out", out, dtype)
@@ -252,11 +255,11 @@ def token_loss(logits, tokens, grad_logprobs, grad_entropy=None, out: TokenLogpr
              _vector("token_loss: grad_logprobs", grad_logprobs, rows, ("f32",)),
              _vector("token_loss: grad_entropy", grad_entropy, rows, ("f32",)))
     if out is None:
-        out = _fresh(rows, tokens, True, 0)
+        out = _fresh(rows, tokens, True, 0, stream)
     elif out.top_tokens is not None or out.top_logprobs is not None:
         raise ValueError("token_loss: the top tokens are token_logprobs'")
     if grad is None:
-        grad = _like(logits, logits.shape, dtype)
+        grad = _new(logits.shape, dtype, stream)
     else:
         _same_shape("token_loss", logits, grad)
     gptr, _, _, gstride = _matrix("token_loss: grad", grad, dtype)
@@ -296,7 +299,7 @@ def grad_norm(grads, out=None, stream=None):
     device."""
     grads = _list(grads)
     if out is None:
-        out = _like(None, [1], "f32")
+        out = _new([1], "f32", stream)
     _run("tc_grad_norm", stream, grads.entries, grads.count, _vector("grad_norm: out", out, 1, ("f32",)))
     return out
 

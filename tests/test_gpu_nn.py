@@ -627,3 +627,67 @@ def test_layer_norm_gradients_where_the_mean_is_near_the_largest_value(device, r
     assert not dw.to_f32().any()
     want = g.sum(0)
     within(db.to_f32(), want, U[dtype] * np.abs(want) + 128 * e * np.abs(g).sum(0))
+
+
+# ---------------------------------------------------------------------------
+# results on a stream of the caller's
+# ---------------------------------------------------------------------------
+def _busy(stream, room):
+    """Some 50 ms of work on `stream`: 100 passes over 3 GB."""
+    for _ in range(100):
+        N.call("tc_memset", room.ptr, 0, room.nbytes, stream)
+
+
+def test_results_are_made_in_their_streams_order(device):
+    """Results that a call on another stream makes come from that stream's
+    order: a block whose last use is queued on the default stream is not
+    written before that use, and one dropped early is not handed to the
+    default stream before the call has written it."""
+    ctx, stream = C.c_void_p(), C.c_void_p()
+    N.call("tc_ctx_create", 0, C.byref(ctx))
+    N.call("tc_ctx_stream", ctx, C.byref(stream))
+    on, shape = stream.value, (2048, 1536)  # 12 MB of f32: a pool class that nothing else here uses
+    room = CudaStorage("bf16", 3 << 29)
+    x = normal(shape, 1)
+    X = tensor(x)
+    want = nn.layer_norm(X)[0].to_numpy()
+    # 1: the default stream is yet to copy from a block that has been dropped
+    old = tensor(normal(shape, 2))
+    kept = old.to_numpy()
+    _busy(None, room)
+    late = old.storage.duplicate()
+    del old
+    y, st = nn.layer_norm(X, stream=on)
+    N.call("tc_stream_sync", on)
+    N.call("tc_stream_sync", None)
+    assert np.array_equal(late.as_slice().reshape(shape), kept)
+    assert np.array_equal(y.to_numpy(), want)
+    # 2: the call's stream is yet to write a result that has been dropped
+    del y, late
+    N.call("tc_stream_sync", None)
+    _busy(on, room)
+    for _ in range(4):
+        nn.layer_norm(X, stream=on)
+    fresh = [CudaStorage.zeros("f32", x.size) for _ in range(4)]
+    N.call("tc_stream_sync", None)
+    N.call("tc_stream_sync", on)
+    for s in fresh:
+        assert not s.as_slice().any()
+    del st, fresh
+    N.call("tc_ctx_destroy", ctx)
+
+
+def test_a_result_may_outlive_its_stream(device):
+    """tc_ctx_destroy waits for the stream; what was made on it stays valid, and
+    goes back to the pool when it is dropped."""
+    ctx, stream = C.c_void_p(), C.c_void_p()
+    N.call("tc_ctx_create", 0, C.byref(ctx))
+    N.call("tc_ctx_stream", ctx, C.byref(stream))
+    X = tensor(normal((300, 700), 1))
+    N.call("tc_stream_sync", None)
+    y, st = nn.layer_norm(X, stream=stream.value)
+    N.call("tc_ctx_destroy", ctx)
+    assert np.array_equal(y.to_numpy(), nn.layer_norm(X)[0].to_numpy())
+    at = y.storage.ptr
+    del y
+    assert CudaStorage("f32", 300 * 700).ptr == at
