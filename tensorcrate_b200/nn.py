@@ -53,6 +53,8 @@ def _matrix(what: str, x, dtype: str | None = None) -> tuple[int, int, int, int]
     for e in shape[:-1]:
         rows *= e
     if type(x) is Tensor:
+        if rows * cols > storage.len:
+            raise ValueError(f"{what}: shape {list(shape)} reaches past {storage.len} elements")
         return storage.ptr, rows, cols, cols
     strides = x.strides
     if cols > 1 and strides[-1] != 1:
@@ -69,6 +71,8 @@ def _matrix(what: str, x, dtype: str | None = None) -> tuple[int, int, int, int]
             elif s != step:
                 raise ValueError(f"{what}: the leading axes {shape[:-1]} do not step as one, call contiguous() first")
             step = s * e
+    if x.offset < 0:
+        raise ValueError(f"{what}: begins before its storage, at element {x.offset}")
     if rows and cols:
         reach = x.offset + (rows - 1) * stride + cols
         if reach > storage.len:
@@ -94,6 +98,8 @@ def _vector(what: str, x, n: int, dtypes: Sequence[str]) -> int | None:
                 raise ValueError(f"{what}: not contiguous")
     if storage.dtype not in dtypes:
         raise ValueError(f"{what}: element type {storage.dtype}, expected {' or '.join(dtypes)}")
+    if offset < 0:
+        raise ValueError(f"{what}: begins before its storage, at element {offset}")
     if held != n or offset + n > storage.len:
         raise ValueError(f"{what}: {held} elements, expected {n}")
     return storage.ptr + offset * _BYTES[storage.dtype]

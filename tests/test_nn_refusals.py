@@ -151,3 +151,24 @@ def test_python_functions_refuse():
         nn.GradList([held([4], "u32")])
     with pytest.raises(ValueError, match="expected 1"):
         nn.clip_grads([x], held([2]), 1.0)
+
+
+def test_what_lies_outside_a_storage_is_refused():
+    """By the host, as the layout checks of the other operators do: a tensor
+    whose shape has more elements than its storage, a view that begins before
+    its storage."""
+    short = Tensor(CudaStorage("f32", 7, ptr=0x1000), [2, 4])
+    before = TensorView(CudaStorage("f32", 64, ptr=0x1000), [2, 4], [4, 1], -8)
+    vector = TensorView(CudaStorage("f32", 64, ptr=0x1000), [4], [1], -1)
+    x, st, tok, u = held([2, 4]), held([2, 2]), held([2], "u32"), held([2])
+    for bad, why in ((short, "past 7 elements"), (before, "before")):
+        for call in (lambda: nn.layer_norm(bad), lambda: nn.layer_norm(x, out=bad), lambda: nn.layer_norm_backward(bad, x, st),
+                     lambda: nn.layer_norm_backward(x, x, st, out=bad), lambda: nn.token_logprobs(bad, tok),
+                     lambda: nn.token_logprobs_backward(x, tok, st, u, out=bad),
+                     lambda: nn.token_loss(x, tok, u, out=nn.TokenLogprobs(), grad=bad)):
+            with pytest.raises(ValueError, match=why):
+                call()
+    with pytest.raises(ValueError, match="before"):
+        nn.layer_norm(x, vector)
+    with pytest.raises(ValueError, match="before"):
+        nn.GradList([vector])
