@@ -58,7 +58,9 @@ def lib(tmp_path_factory):
     objects = [build._compile(build.CSRC / "gradnorm.cu", False, [])]
     (where / "runtime.cpp").write_text(RUNTIME)
     out = where / "lib.so"
-    subprocess.run(["g++", "-shared", "-fPIC", "-O1", "-o", str(out), str(where / "runtime.cpp"), *map(str, objects)], check=True)
+    # -Bsymbolic: its own stand-ins, not a runtime that the process has loaded
+    subprocess.run(["g++", "-shared", "-fPIC", "-O1", "-Wl,-Bsymbolic", "-o", str(out), str(where / "runtime.cpp"),
+                    *map(str, objects)], check=True)
     return C.CDLL(str(out), mode=C.RTLD_LOCAL)
 
 
