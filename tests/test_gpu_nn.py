@@ -691,3 +691,80 @@ def test_a_result_may_outlive_its_stream(device):
     at = y.storage.ptr
     del y
     assert CudaStorage("f32", 300 * 700).ptr == at
+
+
+# ---------------------------------------------------------------------------
+# several turns a block: rows loaded ahead, stages filled again, remainders
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,cols,dtype,pad", [
+    (20011, 64, "bf16", 8), (20011, 64, "f32", 0), (3001, 1001, "f16", 0), (3001, 1001, "f32", 3), (3001, 1001, "bf16", 7),
+    (3001, 4096, "bf16", 0), (1501, 4096, "f32", 4), (1203, 8192, "f16", 8), (1203, 8192, "f32", 0), (701, 16384, "bf16", 0),
+    (301, 16384, "f32", 0), (1203, 5001, "bf16", 0), (603, 5001, "f32", 0), (301, 20001, "bf16", 3)])
+def test_layer_norm_over_many_rows(device, rows, cols, dtype, pad):
+    """More rows than the blocks take in four turns, and no whole number of
+    turns.  Tolerances as in test_layer_norm_and_its_gradients; a column's sum
+    is still less than 128 additions deep: a thread's rows (at most 3001 / 148
+    / 2), its block's groups (15), 148 partial sums over 32 lanes."""
+    eps = 1e-5
+    x = as_type(normal((rows, cols), 1) * 2 + 0.5, dtype)
+    g = as_type(normal((rows, cols), 2), dtype)
+    w, b = as_type(1 + 0.3 * normal(cols, 3), "f32"), as_type(normal(cols, 4), "f32")
+    W, B = tensor(w), tensor(b)
+    X, G, Y = matrix(x, dtype, pad), matrix(g, dtype, pad), blank(rows, cols, dtype, pad)
+    _, st = nn.layer_norm(X, W, B, eps, out=Y)
+    want, mean, rstd, h = norm64(x, w, b, eps)
+    got, kept = read(Y)
+    off = 32 * e * (np.abs(x).mean(1, keepdims=True) + np.abs(mean) + np.abs(x - mean))
+    within(got, want, U[dtype] * np.abs(want) + TINY[dtype] + (off * rstd + 40 * e * np.abs(h)) * np.abs(w) + 4 * e * np.abs(b))
+    assert kept
+    s = st.to_f32().astype(np.float64)
+    within(s[:, :1], mean, off.max(1, keepdims=True))
+    within(s[:, 1:], rstd, rstd * (40 * e + 2 * off.max(1, keepdims=True) * rstd))
+    mean, rstd = s[:, :1], s[:, 1:]
+    D = blank(rows, cols, dtype, pad)
+    _, dw, db = nn.layer_norm_backward(G, X, st, W, out=D)
+    want, want_w, want_b, h, gw = norm_grad64(g, x, w, mean, rstd)
+    got, kept = read(D)
+    deep = 48 * e * rstd * (np.abs(gw) + np.abs(gw).mean(1, keepdims=True) + np.abs(h) * np.abs(gw * h).mean(1, keepdims=True))
+    near = 4 * e * rstd * np.abs(mean) * rstd * (np.abs(gw * h).mean(1, keepdims=True) + np.abs(gw).mean(1, keepdims=True) * np.abs(h))
+    within(got, want, U[dtype] * np.abs(want) + TINY[dtype] + deep + near)
+    assert kept
+    within(dw.to_f32(), want_w, U["f32"] * np.abs(want_w) + 128 * e * (np.abs(g * h) + np.abs(g * mean * rstd)).sum(0))
+    within(db.to_f32(), want_b, U["f32"] * np.abs(want_b) + 128 * e * np.abs(g).sum(0))
+
+
+@pytest.mark.parametrize("rows,vocab,dtype,mask,pad", [
+    (80003, 33, "f16", "none", 0), (80003, 33, "f32", "inf", 3), (3001, 4104, "bf16", "inf", 0), (3001, 4104, "f16", "lowest", 8),
+    (1801, 8200, "f32", "none", 0), (1801, 8200, "f32", "lowest", 4), (2003, 5003, "f16", "inf", 0), (1601, 16411, "bf16", "none", 0)])
+def test_token_loss_over_many_rows(device, rows, vocab, dtype, mask, pad):
+    """More rows than are resident at once: a warp or a block goes on to
+    others, the next row copied while this one's gradient is written.
+    Tolerances as in test_token_logprobs_and_their_gradients."""
+    rng = np.random.default_rng(vocab)
+    x = as_type(masked(rng.standard_normal((rows, vocab)).astype(np.float32) * 3 + 20, mask, dtype, rng), dtype)
+    token = rng.integers(0, vocab, rows).astype(np.uint32)
+    token[2::7] = N.NO_TOKEN
+    tok = CudaStorage.store(token, "u32")
+    u, v = as_type(rng.standard_normal(rows), "f32"), as_type(rng.standard_normal(rows), "f32")
+    u[5::9] = v[5::9] = 0.0
+    X = matrix(x, dtype, pad)
+    lp, ent, m, ls = tokens64(x, token)[:4]
+    for with_entropy in (True, False):
+        v_ = v if with_entropy else np.zeros(rows)
+        want, p, a, ent_, u_, one = slope64(x, token, u, v_)
+        with np.errstate(invalid="ignore", over="ignore"):
+            size = p * (np.abs(u_) + np.abs(v_[:, None]) * (1 + np.where(p > 0, np.abs(a), 0.0) + ent_[:, None])) + np.abs(u_) * one
+        F = blank(rows, vocab, dtype, pad)
+        out, _ = nn.token_loss(X, tok, tensor(u), tensor(v) if with_entropy else None, grad=F,
+                               out=None if with_entropy else nn.TokenLogprobs(tensor(np.zeros(rows))))
+        got, kept = read(F)
+        within(got, want, U[dtype] * np.abs(want) + TINY[dtype] + 2.0 ** -16 * size + 1e-37)
+        assert kept
+        with np.errstate(invalid="ignore"):
+            within(out.logprobs.to_f32(), lp, 2.0 ** -18 + 4 * e * (np.abs(np.where(np.isfinite(lp), lp, 0.0)) + 2 * ls))
+        if with_entropy:
+            within(out.entropy.to_f32(), ent, 2.0 ** -17 * (1 + ent + ls))
+            assert np.array_equal(out.statistics.to_f32()[:, 0], m)
+    if vocab < 100:
+        got = nn.token_logprobs(X, tok, top=3)
+        assert np.array_equal(got.top_tokens.to_numpy(), np.argsort(-x, axis=1, kind="stable")[:, :3])

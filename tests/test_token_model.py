@@ -124,3 +124,32 @@ def test_tape_rules_refuse():
     N.call("tc_tape_destroy", out)
 
 
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_the_models_clipped_gradients_are_within_the_limit(device, dtype, monkeypatch):
+    """In every step of the model: the norm of what Adam is given is at most
+    the limit, and the limit itself where the norm before was above it.  Each
+    gradient is rounded once to its type, the factor and the norm to f32."""
+    from tensorcrate_b200 import token_model
+
+    seen, clip = [], token_model.nn.clip_grads
+
+    def watched(grads, norm, limit, stream=None):
+        clip(grads, norm, limit, stream)
+        clipped = [g.to_f32().astype(np.float64) for g in grads._keep[0]]
+        seen.append((float(norm.to_f32()[0]), np.sqrt(sum((g ** 2).sum() for g in clipped))))
+
+    monkeypatch.setattr(token_model.nn, "clip_grads", watched)
+    rng = np.random.default_rng(7)
+    limit, vocab, rows = 0.05, 257, 64
+    model = TokenModel(32, 128, vocab, dtype=dtype, limit=limit, rate=1e-2)
+    x = cuda.CudaStorage.store(O.narrow(rng.standard_normal(rows * 32).astype(np.float32), dtype), dtype)
+    tokens = cuda.CudaStorage.store(rng.integers(0, vocab, rows).astype(np.uint32), "u32")
+    for _ in range(6):
+        model.step(x, tokens)
+    near = 4 * 2.0 ** -24 + {"f32": 2.0 ** -24, "bf16": 2.0 ** -8}[dtype]
+    assert len(seen) == 6 and any(before > limit for before, _ in seen)
+    for before, after in seen:
+        assert abs(after - min(before, limit)) <= near * limit
