@@ -16,7 +16,8 @@ class Tape:
     def __init__(self, dtype: str = "f32", stream=None):
         self.dtype = dtype
         out = C.c_void_p()
-        N.call("tc_tape_create", N.DTYPES[dtype], _stream(stream), C.byref(out))
+        self._on = _stream(stream)  # what the tape records, reads and frees is in this stream's order
+        N.call("tc_tape_create", N.DTYPES[dtype], self._on, C.byref(out))
         self.handle = out
         self._keep = []  # leaves' storages outlive the tape's reads
 
@@ -84,7 +85,7 @@ class Tape:
             return None
         n = int(np.prod(self.shape(v))) if self.shape(v) else 1
         out = np.empty(n, ELEM[self.dtype][0])
-        N.call("tc_stream_sync", None)
+        N.call("tc_stream_sync", self._on)
         N.call("tc_memcpy_d2h", out.ctypes.data, ptr, out.nbytes, None)
         return out.reshape(self.shape(v)) if self.shape(v) else out
 
@@ -101,7 +102,7 @@ class Tape:
         return CudaStorage(self.dtype, int(np.prod(shape, dtype=np.int64)), ptr=ptr) if ptr else None
 
     def value_storage(self, v: int) -> CudaStorage:
-        """A var's value on the device, the tape's."""
+        """A var's value on the device, the tape's, in its stream's order."""
         p = C.c_void_p()
         N.call("tc_tape_value", self.handle, v, C.byref(p), None, None)
         return self._storage(p.value, v)
@@ -120,13 +121,15 @@ class Tape:
 
     def close(self) -> None:
         if self.handle:
-            N.call("tc_stream_sync", None)
+            N.call("tc_stream_sync", self._on)
             N.call("tc_tape_destroy", self.handle)
             self.handle = None
 
     def __del__(self):
         try:
             if self.handle and N._lib is not None:
+                if self._on is not None:  # the leaves go back in the default stream's order
+                    N._lib.tc_stream_sync(self._on)
                 N._lib.tc_tape_destroy(self.handle)
         except Exception:
             pass

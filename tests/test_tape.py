@@ -124,3 +124,37 @@ def test_half_types_round_each_rule(device, dtype):
     assert np.max(np.abs(gx - want_x)) <= 4 * step * np.max(np.abs(want_x))
     assert np.max(np.abs(gw - want_w)) <= 4 * step * np.max(np.abs(want_w))
     t.close()
+
+
+@pytest.mark.gpu
+def test_values_of_a_tape_on_its_own_stream(device):
+    """A tape records on the stream it was made with: values, adjoints and the
+    end of its leaves wait for that stream, not for the default one."""
+    import ctypes as C
+
+    from tensorcrate_b200 import _native as N
+
+    ctx, stream = C.c_void_p(), C.c_void_p()
+    N.call("tc_ctx_create", 0, C.byref(ctx))
+    N.call("tc_ctx_stream", ctx, C.byref(stream))
+    room = cuda.CudaStorage("bf16", 3 << 29)
+    x, g, b = normal((64, 3000), 1), 1 + 0.1 * normal(3000, 2), normal(3000, 3)
+    token = np.arange(64, dtype=np.uint32)
+
+    def results(on):
+        tape = Tape("f32", stream=on)
+        leaves = [tape.leaf(cuda.CudaStorage.store(v.ravel(), "f32"), list(v.shape)) for v in (x, g, b)]
+        N.call("tc_stream_sync", None)
+        for _ in range(100):  # the tape's kernels run some 50 ms later
+            N.call("tc_memset", room.ptr, 0, room.nbytes, on)
+        loss = tape.token_loss(tape.layer_norm(*leaves), cuda.CudaStorage.store(token, "u32"), 1.0 / 64)
+        value = tape.value(loss).copy()
+        tape.backward(loss)
+        grads = [tape.grad(v) for v in leaves]
+        tape.close()
+        return [value, *grads]
+
+    want = results(None)
+    for a, w in zip(results(stream.value), want):
+        assert np.array_equal(a, w)
+    N.call("tc_ctx_destroy", ctx)
