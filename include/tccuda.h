@@ -454,7 +454,9 @@ int tc_layer_norm(int dtype, int param_dtype, size_t rows, size_t cols, const vo
 /* The gradients of tc_layer_norm from the gradient `grad` of y and the
  * forward pass's x and statistics: grad_x (may be grad or x, with the same
  * stride), and grad_weight and grad_bias of `param_dtype`, summed over the
- * rows in an order that depends on the sizes alone.  Any of the three may be
+ * rows in an order that the sizes, the device and whether pointers and strides
+ * lie on the 16-byte grid give: the same call on the same buffers gives the
+ * same bits, on buffers aligned otherwise it may not.  Any of the three may be
  * NULL: it is not computed.  The sums use the stream's scratch. */
 int tc_layer_norm_backward(int dtype, int param_dtype, size_t rows, size_t cols, const void *grad,
                            size_t grad_stride, const void *x, size_t x_stride, const float *statistics,
@@ -510,8 +512,9 @@ typedef struct tc_gradient {
   int dtype;
 } tc_gradient;
 /* norm[0] = the square root of the sum of every gradient's squares, in f64,
- * added in an order that depends on the sizes alone, rounded once to f32.  `out` is not
- * used.  Uses the stream's scratch. */
+ * rounded once to f32.  They are added in an order that the sizes, each
+ * address modulo 128 and the device give: the same buffers give the same bits,
+ * buffers aligned otherwise may not.  `out` is not used.  Uses the stream's scratch. */
 int tc_grad_norm(const tc_gradient *grads, size_t count, float *norm, void *stream);
 /* out = g * min(1, limit / norm[0]), the factor in f32.  norm is read on the
  * device, so a caller may first combine the norms of several ranks.  A norm

@@ -713,8 +713,10 @@ enum Extra { NOTHING = 0, TOP = 1, GRADIENT = 2 };
 
 // Small vocabularies: a warp holds a row, U runs a lane.  The row is read
 // once, whatever is asked for but the top tokens' second look.  Bound by
-// issue: 65536x1000 bf16 with entropy in 34 us (floor 20), with 5 top tokens
-// in 116; the loss of 65536x1024 in 59 (floor 42).
+// issue: 67108x1000 bf16 with entropy in 34 us (floor 21), with 5 top tokens
+// in 131; the loss of 65536x1024 with entropy in 64 (floor 42).  Blocks of a
+// row each take 118, 361 and 235; at 2048 tokens, the most that a warp holds,
+// 32768 rows take 34 us for 73, and 73 for 139 with the loss.
 template <class T, bool ENT, int EXTRA, int U> __global__ void __launch_bounds__(256) token_small(const TokenArgs a) {
   using S = typename T::S;
   constexpr unsigned V = Cut<T>::V;
@@ -857,7 +859,7 @@ template <class T> struct Ahead {
 // rows copied ahead through shared memory took 58 us for 56).  8192x32768 bf16
 // with entropy in 93 us, 5.8 TB/s; 2048x50257 in 44 us, where 2.3 rounds of
 // blocks begin and end together.  With top tokens the steps between the row's
-// barriers, not HBM, take the time: 66 us with 8 of them, some rows masked to
+// barriers, not HBM, take the time: 67 us with 8 of them, some rows masked to
 // nothing.  (Their code spills with the registers of six blocks an SM: 77 us;
 // five are kept.)
 template <class T, bool ENT, int EXTRA> __global__ void __launch_bounds__(256, EXTRA == TOP ? 5 : 6) token_rows(const TokenArgs a) {
@@ -915,7 +917,9 @@ template <class T, bool ENT, int EXTRA> __global__ void __launch_bounds__(256, E
 
 // The loss of rows that a block's shared memory holds: a row stays in its
 // slots until its gradient is written from there, and the next one follows it
-// group by group.  16384x8192 bf16 in 108 us, 5.0 TB/s (138 us read twice).
+// group by group.  Against rows read twice (token_loss_twice), without entropy:
+// f32 87 us for 98 at 16384x4096, 94 for 97 at 4096x16384; bf16 213 for 239 at
+// 53687x2500, 107 for 103 at 16384x8192, 104 for 103 at 4096x32768.
 template <class T, bool ENT> __global__ void __launch_bounds__(256, 3) token_loss_held(const TokenArgs a, unsigned groups) {
   using S = typename T::S;
   constexpr unsigned V = Cut<T>::V;
@@ -971,7 +975,7 @@ template <class T, bool ENT> __global__ void __launch_bounds__(256, 3) token_los
 // Larger rows, and few: the blocks of a cluster share a row, and the second
 // pass reads it from L2, which the parts of all resident blocks leave room in
 // (2.1 GB of HBM traffic at 4096x131072 bf16, where blocks of whole rows made
-// it 3.1).  420 us, 5.1 TB/s: the two passes' exponentials keep the special
+// it 3.1).  421 us, 5.1 TB/s: the two passes' exponentials keep the special
 // function unit 60% busy between the row's barriers.
 template <class T, bool ENT> __global__ void __launch_bounds__(256, 4) token_loss_twice(const TokenArgs a) {
   using S = typename T::S;
@@ -996,8 +1000,9 @@ template <class T, bool ENT> __global__ void __launch_bounds__(256, 4) token_los
 }
 
 // The gradient alone, from the statistics that the forward call left, by
-// blocks or (`apart`) by warps of a row each.  Bound by HBM: 4096x32768 f32
-// with entropy in 168 us, 6.4 TB/s.
+// blocks or (`apart`) by warps of a row each.  Bound by HBM: with entropy
+// 4096x32768 f32 in 168 us, 6.4 TB/s; bf16 8192x32768 in 169, 6.3 TB/s, and
+// 5341x50257 in 177, 6.1.
 template <class T, bool ENT> __global__ void __launch_bounds__(512) token_slope(const TokenArgs a, bool apart) {
   using S = typename T::S;
   const unsigned threads = apart ? 32 : blockDim.x, each = blockDim.x / threads;
@@ -1052,9 +1057,11 @@ unsigned parts_for(size_t rows, size_t runs, unsigned threads, size_t slots) {
 }
 
 // The most runs of a part whose row is read twice: 100 KB a block, of which
-// four blocks on each of 148 SMs hold 60 MB. 4096x131072 bf16 (16384 runs)
-// takes 411 us in four parts, 462 in two, 476 in one; 4096x50257 (6282) 175
-// in one, 181 in two.
+// four blocks on each of 148 SMs hold 60 MB.  In one, two and four parts, 2^28
+// bf16 logits: 218, 239, 364 us at 50257 tokens (6282 runs); 218, 224, 333 at
+// 53248 (6656); 218, 230, 318 at 57344; 231, 209, 265 at 65536 (8192); 245, 215,
+// 242 at 98304; 256, 241, 230 at 131072.  So between 6400 and some 7500 runs two
+// parts lose up to 5%.
 constexpr size_t PART_RUNS = 6400;
 // A warp a row up to 8 runs a lane; 2 or 4 where those do.
 template <class T, bool ENT, int EXTRA> int small(const char *what, const TokenArgs &a, cudaStream_t stream) {
@@ -1071,7 +1078,13 @@ template <class T, bool ENT, bool WITH_TOP> int forward(const TokenArgs &a, cuda
   if (is_small<T>(a)) return small<T, ENT, EXTRA>("token logprobs", a, stream);
   auto kernel = token_rows<T, ENT, EXTRA>;
   const size_t runs = a.vocab / Cut<T>::V;
-  // the top tokens' steps wait for one another: smaller blocks, more of them
+  // Blocks of 128 threads have less to join a row, those of 256 more loads
+  // ahead: 90 us for 107 at 16384x16384 bf16, 91 for 93 at 8192x32768, 106 for 92
+  // at 2048x131072; f32 84 for 95 at 16384x8192 (2048 runs, as 16384 of 16
+  // bits), 87 for 86 at 8192x16384.  The top tokens' steps wait for one another,
+  // so many rows take smaller blocks, more of them: 8 of 2048x16384 bf16 in 31 us
+  // for 34 (but 64 for 61 at 50257 and 137 for 111 at 131072); up to a row an SM
+  // the larger ones, 14 for 22 us at 148x16384.
   const unsigned threads = runs >= 2048 && (!WITH_TOP || a.rows <= size_t(sm_count())) ? 256 : 128;
   const size_t slots = resident(kernel, threads, 0);
   const unsigned parts = parts_for(a.rows, runs, threads, slots);
@@ -1081,6 +1094,9 @@ template <class T, bool ENT, bool WITH_TOP> int forward(const TokenArgs &a, cuda
 template <class T, bool ENT> int loss(const TokenArgs &a, cudaStream_t stream) {
   if (is_small<T>(a)) return small<T, ENT, GRADIENT>("token loss", a, stream);
   const size_t runs = a.vocab / Cut<T>::V;
+  // 128 threads for 256: bf16 206 us for 282 at 32768x8192, 193 for 222 at
+  // 16384x16384 (2048 runs), 236 for 206 at 8192x32768; f32 189 for 192 at
+  // 16384x8192 (2048), 230 for 174 at 8192x16384.
   const unsigned threads = runs >= 2048 ? 256 : 128;
   // Sixteen runs a thread leave three blocks on an SM; with fewer rows than
   // SMs each row is better shared.
@@ -1102,6 +1118,9 @@ template <class T, bool ENT> int loss(const TokenArgs &a, cudaStream_t stream) {
 template <class T, bool ENT> int backward(const TokenArgs &a, cudaStream_t stream) {
   const bool apart = is_small<T>(a);
   const size_t runs = a.vocab / Cut<T>::V;
+  // 128, 256 and 512 threads, 2^28 bf16 logits: 184, 226, 392 us at 8192 tokens
+  // (1024 runs), 167, 183, 228 at 16384 (2048), 173, 169, 185 at 32768, 177, 172,
+  // 170 at 65536 (8192).
   const unsigned threads = apart ? 256 : runs >= 8192 ? 512 : runs >= 2048 ? 256 : 128;
   const size_t blocks = apart ? (a.rows + 7) / 8 : a.rows;
   token_slope<T, ENT><<<unsigned(std::min<size_t>(blocks, 1u << 30)), threads, 0, stream>>>(a, apart);

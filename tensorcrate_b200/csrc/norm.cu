@@ -18,10 +18,13 @@ namespace {
 // A row's elements stay in the registers of the threads that share it (a
 // warp's up to 1024 columns, else a block's), so x is read once for both of
 // the variance's passes.  Access k of thread t covers the E elements from (t
-// + k * threads) * E: neighbours read neighbouring addresses.  f32 rows are
-// bound by HBM: 32768x1024 in 48 us, 5.6 TB/s (43 us of it the kernel's); rows
-// off the 16-byte grid (E = 1) by their single accesses, 65536x1001 bf16 in
-// 108 us, 38% of the floor.
+// + k * threads) * E: neighbours read neighbouring addresses.  A warp a row
+// against a block: 59 us for 74 at 131072x256 f32, 115 for 148 at 65536x1001
+// bf16, 48 for 47 at 32768x1024 f32.  f32 rows are bound by HBM: 32768x1024 in
+// 48 us, 5.6 TB/s (43 us of it the kernel's).  Rows off the 16-byte grid (E =
+// 1) are bound by their single accesses: 67041x1001 bf16 in 117 us, 35% of the
+// floor; past 1024 columns their 16 elements a thread spill as well (12 to 32
+// bytes): 13419x5001 bf16 in 165 us, 25%.
 template <class T, class P, int E, int K, bool WARP>
 __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_rows(const typename T::S *x, size_t x_stride,
                                                   const typename P::S *__restrict__ w,
@@ -88,8 +91,9 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) norm_rows(const typename T:
 // every row, whose weights and biases they keep in registers; the next
 // turn's rows are loaded before this one's are used.  16384x8192 bf16 with f32
 // weights in 109 us, 4.9 TB/s (169 us by blocks of a row each that read the
-// weights again); 32768x4096 103, 5.2 TB/s (156); 65536x1024 54 (60).  Single
-// elements of rows off the grid gain nothing by it (65536x1001: 152 us for
+// weights again); 32768x4096 103, 5.2 TB/s (156); 65536x1024 54 (60).  Rows of
+// 8192 to 16384 columns, at 32 a thread, spill 80 bytes: 8192x16384 in 153 us,
+// 54% of the floor.  Single elements of rows off the grid gain nothing by it (65536x1001: 152 us for
 // 108), they stay with norm_rows.
 struct NormTurns {
   const void *x, *w, *b;
@@ -220,7 +224,8 @@ __global__ void __launch_bounds__(MOST, BLOCKS) norm_turns(const NormTurns a) {
 }
 
 // Rows of more than 16384 columns: a block reads its row three times, the
-// second and third from L2.
+// second and third from L2, by single elements: 8192x20000 bf16 in 538 us (19%
+// of the floor), 4096x20000 f32 in 306 (33%).
 template <class T, class P>
 __global__ void __launch_bounds__(1024) norm_rows_wide(const typename T::S *x, size_t x_stride,
                                                        const typename P::S *__restrict__ w,
@@ -277,14 +282,17 @@ __global__ void __launch_bounds__(1024) norm_rows_wide(const typename T::S *x, s
 // of 16 warps, all in step, with too little between them.
 //
 // What bounds it: the one block that an SM's registers hold, 16 warps that
-// issue half of the time (of the HBM floor: f32 rows 93% up to 4096 columns,
-// 16-bit rows 78 to 82% there and 73% at 8192); past 8192 columns the
-// clusters' barriers too (61% at 16384, where 32 columns a thread spilled and
-// reached 28%), and off the 16-byte grid the single 2-byte accesses (47% at
-// 1001 columns).  16384x8192 bf16, 805 MB: 170 us for this kernel and 182
-// us a call, 4.4 TB/s (one row a turn: 186 us a call; 1024 threads of 8
+// issue half of the time (of the HBM floor: f32 rows 92% up to 4096 columns,
+// 16-bit rows 90% up to 1024, 77% at 4096 and 72% at 8192); past 8192 columns
+// the clusters' barriers too (60% at 16384, where 32 columns a thread spilled
+// and reached 28%).  16384x8192 bf16, 805 MB: 168 us for this kernel and 171 to
+// 181 a call, 4.6 TB/s (one row a turn: 186 us a call; 1024 threads of 8
 // columns each spill: 289 us; rows through registers without the ring: 263
-// us); 2048x4096 bf16 24.6 us, 4099x1001 f16 18.0 us a call.
+// us); 2048x4096 bf16 24.6 us a call.  Off the 16-byte grid it is the single
+// accesses to shared memory and of the stores, 46% at 67041x1001 bf16 (8
+// columns a thread: 75 us at 33520x1001 where 16 take 91, 83 for 98 at
+// 8386x4001); past 4096 columns a thread's 16 spill 28 to 68 bytes as well, 25%
+// at 13419x5001 bf16.
 struct NormGrad {
   const void *g, *x, *w;
   size_t g_stride, x_stride, dx_stride, rows;
@@ -550,7 +558,9 @@ __global__ void __launch_bounds__(512) norm_grad_rows(const NormGrad a) {
   }
 }
 
-// Rows of more than 32768 columns: grad_x by blocks that read their row twice ...
+// Rows of more than 32768 columns, by single elements (2048x40000 bf16 in 470
+// us, 16% of the floor; 1024x65536 f32 in 517, 24%): grad_x by blocks that read
+// their row twice ...
 template <class T, class P>
 __global__ void __launch_bounds__(1024) norm_grad_wide(const typename T::S *g, size_t g_stride,
                                                        const typename T::S *x, size_t x_stride,
@@ -602,8 +612,8 @@ __global__ void __launch_bounds__(128) norm_grad_columns(const typename T::S *g,
   partial[size_t(blockIdx.y) * 2 * cols + cols + c] = sb;
 }
 
-// grad_w and grad_b from the blocks' partial sums, in an order that the sizes
-// give: 32 columns a block, each of its 32 warps a part of the partials.  The
+// grad_w and grad_b from the blocks' partial sums, in an order that their
+// number gives: 32 columns a block, each of its 32 warps a part of the partials.  The
 // block may be resident before the partials are written; it waits for them
 // where it says so.
 template <class P>
