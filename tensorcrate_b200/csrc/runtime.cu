@@ -213,6 +213,21 @@ size_t size_class(size_t bytes) {
   return (bytes + two_mib - 1) / two_mib * two_mib;
 }
 
+// While it lives this thread may ask after events and allocate though it
+// captures a stream: what the pool does is no part of the graph.
+struct BesideCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  BesideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~BesideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+// Whether `stream` is being captured: it cannot wait for work outside its
+// graph, and an event recorded on it stands for no point in time.
+bool capturing(cudaStream_t stream) {
+  if (!stream) return false;
+  cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
+  return cudaStreamIsCapturing(stream, &s) == cudaSuccess && s != cudaStreamCaptureStatusNone;
+}
+
 // A cached block of class `cls` on `dev` that a request may take (with the
 // pool's lock held).  `stream` is the requesting stream, or has_stream false
 // for tc_malloc.  On success the block is live and, when it was freed on
@@ -233,7 +248,7 @@ bool take_cached(Pool &p, int dev, size_t cls, bool has_stream, cudaStream_t str
     for (int i = int(v.size()) - 1; i >= 0 && pick < 0; --i) {
       const FreeBlock &f = v[size_t(i)];
       if (pass == 0 ? ordered(f.uses[0]) && ordered(f.uses[1])
-                    : pass == 1 ? finished(f.uses[0]) && finished(f.uses[1]) : has_stream)
+                    : pass == 1 ? finished(f.uses[0]) && finished(f.uses[1]) : has_stream && !capturing(stream))
         pick = i;
     }
   }
@@ -260,6 +275,7 @@ int pool_malloc(void **out, size_t bytes, bool has_stream, cudaStream_t stream) 
   if (int st = current_device(&dev)) return st;
   size_t cls = size_class(bytes);
   Pool &p = pool();
+  BesideCapture beside;
   {
     std::lock_guard<std::mutex> g(p.mu);
     if (take_cached(p, dev, cls, has_stream, stream, out)) return TC_OK;
@@ -308,7 +324,7 @@ int pool_free(void *dev_ptr, bool has_stream, cudaStream_t stream, bool with_hom
   const uintptr_t key = reinterpret_cast<uintptr_t>(stream);
   if (has_stream)
     if (int st = record_use(p, key, &f.uses[0])) return st;
-  if (with_home && b.has_home && b.home != key)
+  if (with_home && b.has_home && b.home != key && !capturing(reinterpret_cast<cudaStream_t>(b.home)))
     if (int st = record_use(p, b.home, &f.uses[1])) {
       if (f.uses[0].done) p.spare_events.push_back(f.uses[0].done);
       return st;

@@ -768,3 +768,34 @@ def test_token_loss_over_many_rows(device, rows, vocab, dtype, mask, pad):
     if vocab < 100:
         got = nn.token_logprobs(X, tok, top=3)
         assert np.array_equal(got.top_tokens.to_numpy(), np.argsort(-x, axis=1, kind="stable")[:, :3])
+
+
+def test_results_made_while_the_stream_is_captured(device):
+    """A call on a stream that is captured into a CUDA graph makes its results
+    as any other, where a call of the same size went before: from the pool or
+    anew, without waiting for or asking after work outside the capture."""
+    import torch
+
+    X, W = tensor(normal((40, 600), 1)), tensor(normal(600, 2))
+    other = tensor(normal((40, 600), 3))
+    want = [t.to_numpy() for t in nn.layer_norm(other, W)]
+    cap, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    nn.layer_norm(X, W, stream=cap)
+    torch.cuda.synchronize()
+    # the pool's blocks of these sizes: last used on the stream, on the default one, none
+    for freed_on in (cap, None, "nothing"):
+        graph = torch.cuda.CUDAGraph()
+        if freed_on == "nothing":
+            hold = [CudaStorage("f32", n) for n in (24000, 80) for _ in range(20)]
+        elif freed_on is None:
+            _ = [nn.layer_norm(X, W) for _ in range(8)]
+            del _
+        with torch.cuda.graph(graph, stream=cap):
+            y, st = nn.layer_norm(X, W, stream=cap)
+            nn.layer_norm(y, W, stream=cap)  # a result dropped at once
+            nn.layer_norm(X, W, out=y, statistics=st, stream=cap)
+        N.call("tc_memcpy_d2d", X.storage.ptr, other.storage.ptr, X.storage.nbytes, None)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(y.to_numpy(), want[0]) and np.array_equal(st.to_numpy(), want[1])
+        del graph, y, st
